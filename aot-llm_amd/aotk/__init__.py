@@ -10,7 +10,8 @@ fallback: a missing library raises AotkError.
 from . import abi, configs  # noqa: F401
 from .abi import AotkError  # noqa: F401
 from .runtime import (  # noqa: F401
-    DeviceBuffer, Model, Sampler, copy_dev, State, Weight, argmax, attention, dequant_rows, gelu_mul, init, matmul, matmul2, matmul_noalloc, matvec, matvec2, matvec3,
-    matvec_f32, quantize_q8_0, quantize_q8_k, quantize_rows, rmsnorm, rmsnorm_heads, rope, silu_mul, softmax,
+    LOGITS_RULE_DTYPE, NO_TOKEN, DeviceBuffer, Model, Sampler, copy_dev, State, Weight, allowed_mask, argmax, attention,
+    attention_shared, attention_sinks, dequant_rows, gelu_mul, init, logits_rules, logits_rules_table, matmul, matmul2,
+    matmul_noalloc, matvec, matvec2, matvec3, matvec_f32, quantize_q8_0, quantize_q8_k, quantize_rows, rmsnorm, rmsnorm_heads, rope, silu_mul, softmax,
     stream, sync, time_hbm, time_matvec, time_matmul,
 )

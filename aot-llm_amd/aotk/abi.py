@@ -80,7 +80,14 @@ class SamplerConfig(C.Structure):
                 ("repeat_last_n", C.c_uint32), ("reserved", C.c_uint32), ("seed", C.c_uint64)]
 
 
+class LogitsRule(C.Structure):
+    """aotk_logits_rule: the rules of one row of logits."""
+    _fields_ = [("repetition", C.c_float), ("presence", C.c_float), ("frequency", C.c_float), ("hist_off", C.c_uint32),
+                ("hist_len", C.c_uint32), ("bias_off", C.c_uint32), ("bias_len", C.c_uint32), ("mask", C.c_int32)]
+
+
 assert C.sizeof(Tensor) == 40
+assert C.sizeof(LogitsRule) == 32
 assert C.sizeof(Layer) == 16 * 40 + 8
 
 
@@ -140,6 +147,9 @@ def load(path=None):
     _sig(lib, "aotk_gelu_mul", i, [vp, vp, sz])
     _sig(lib, "aotk_add", i, [vp, vp, sz])
     _sig(lib, "aotk_attention", i, [vp, vp, vp, vp, sz, sz, sz, sz, sz, sz, sz, sz])
+    _sig(lib, "aotk_attention_sinks", i, [vp, vp, vp, vp, i, sz, sz, sz, sz, sz, sz, sz, sz, sz])
+    _sig(lib, "aotk_attention_shared", i, [vp, vp, vp, vp, vp, vp, i, sz, sz, sz, sz, sz, sz, sz, sz, vp, vp])
+    _sig(lib, "aotk_logits_rules", i, [vp, vp, i, sz, sz, sz, vp, vp, sz, vp, vp, sz, vp, sz, vp])
     _sig(lib, "aotk_argmax", i, [vp, sz, C.POINTER(u32)])
     _sig(lib, "aotk_model_load", vp, [C.POINTER(ModelSpec), vp, sz])
     _sig(lib, "aotk_model_synthetic", vp, [C.POINTER(ModelSpec), u64])
@@ -151,6 +161,7 @@ def load(path=None):
     _sig(lib, "aotk_forward", i, [vp, u32, sz, i])
     _sig(lib, "aotk_forward_batch", i, [vp, C.POINTER(u32), sz, sz, i])
     _sig(lib, "aotk_logits", i, [vp, fp])
+    _sig(lib, "aotk_logits_dev", vp, [vp])
     _sig(lib, "aotk_greedy", i, [vp, C.POINTER(u32)])
     _sig(lib, "aotk_generate_greedy", i, [vp, sz, sz, C.POINTER(u32)])
     _sig(lib, "aotk_kv_download", i, [vp, sz, fp, fp])

@@ -267,6 +267,108 @@ def attention(q, k_cache, v_cache, n_head, n_kv_head, head_dim, ctx, layer, pos0
     return out.to_numpy(np.float32)
 
 
+FLOAT_DTYPES = {abi.F32: np.dtype("<f4"), abi.F16: np.dtype("<f2"), abi.BF16: np.dtype("<u2")}  # bf16 as its bits
+LOGITS_RULE_DTYPE = np.dtype([("repetition", "<f4"), ("presence", "<f4"), ("frequency", "<f4"), ("hist_off", "<u4"),
+                              ("hist_len", "<u4"), ("bias_off", "<u4"), ("bias_len", "<u4"), ("mask", "<i4")])
+NO_TOKEN = 0xFFFFFFFF  # the pick of a row whose rules leave no token
+
+
+def _dev(a, dtype):
+    a = np.ascontiguousarray(a)
+    if a.dtype != dtype:
+        raise TypeError(f"expected {dtype} values, got {a.dtype}")
+    return DeviceBuffer.from_numpy(a)
+
+
+def attention_sinks(q, k_cache, v_cache, n_head, n_kv_head, head_dim, ctx, layer, pos0, m, window, n_sink, kind=abi.F32):
+    """Attention of m rows over a sliding window and the first n_sink
+    positions (aotk_attention_sinks); bf16 arrays as uint16 bits."""
+    t = FLOAT_DTYPES[kind]
+    dq, dk, dv = _dev(q, t), _dev(k_cache, t), _dev(v_cache, t)
+    n = m * n_head * head_dim
+    assert n * t.itemsize <= dq.nbytes, "q is smaller than its rows"
+    need = (layer + 1) * ctx * n_kv_head * head_dim * t.itemsize
+    assert need <= dk.nbytes and need <= dv.nbytes, "a cache is smaller than its layers"
+    out = DeviceBuffer(n * t.itemsize)
+    abi.check(_lib().aotk_attention_sinks(out.ptr, dq.ptr, dk.ptr, dv.ptr, kind, n_head, n_kv_head, head_dim, ctx, layer,
+                                          pos0, m, window, n_sink))
+    return out.to_numpy(t)
+
+
+def attention_shared(q, k_prefix, v_prefix, k_tail, v_tail, n_head, n_kv_head, head_dim, prefix_ctx, n_prefix, tail_ctx,
+                     layer, tail_len, rows=None, kind=abi.F32):
+    """Attention of a batch of sequences behind one prefix
+    (aotk_attention_shared); rows None = one row each."""
+    t = FLOAT_DTYPES[kind]
+    lens = np.ascontiguousarray(tail_len, np.uint32)
+    nr = None if rows is None else np.ascontiguousarray(rows, np.uint32)
+    assert nr is None or nr.size == lens.size, "tail_len and rows differ in length"
+    total = lens.size if nr is None else int(nr.sum(dtype=np.uint64))
+    bufs = [_dev(a, t) for a in (q, k_prefix, v_prefix, k_tail, v_tail)]
+    n, kv = total * n_head * head_dim, n_kv_head * head_dim
+    assert n * t.itemsize <= bufs[0].nbytes, "q is smaller than its rows"
+    for b, need in zip(bufs[1:], [prefix_ctx] * 2 + [lens.size * tail_ctx] * 2):
+        assert (layer + 1) * need * kv * t.itemsize <= b.nbytes, "a cache is smaller than its layers"
+    out = DeviceBuffer(n * t.itemsize)
+    abi.check(_lib().aotk_attention_shared(out.ptr, *[b.ptr for b in bufs], kind, n_head, n_kv_head, head_dim, prefix_ctx,
+                                           n_prefix, tail_ctx, layer, lens.size, _np_ptr(lens),
+                                           None if nr is None else _np_ptr(nr)))
+    return out.to_numpy(t)[:n]
+
+
+def logits_rules_table(rules):
+    """(table, history, bias ids, biases) of aotk_logits_rules from one dict
+    per row: repetition, presence, frequency, history (token ids), bias ({id:
+    value} or (id, value) pairs), mask (row of the masks, -1 = none)."""
+    table = np.zeros(len(rules), LOGITS_RULE_DTYPE)
+    hist, ids, vals = [], [], []
+    for row, r in zip(table, rules):
+        unknown = set(r) - {"repetition", "presence", "frequency", "history", "bias", "mask"}
+        if unknown:
+            raise ValueError(f"unknown rules {sorted(unknown)}")
+        bias = r.get("bias", ())
+        bias = list(bias.items()) if isinstance(bias, dict) else list(bias)
+        h = list(r.get("history", ()))
+        row["repetition"], row["presence"] = r.get("repetition", 1.0), r.get("presence", 0.0)
+        row["frequency"], row["mask"] = r.get("frequency", 0.0), r.get("mask", -1)
+        row["hist_off"], row["hist_len"], row["bias_off"], row["bias_len"] = len(hist), len(h), len(ids), len(bias)
+        hist += h
+        ids += [i for i, _ in bias]
+        vals += [v for _, v in bias]
+    return table, np.array(hist, np.uint32), np.array(ids, np.uint32), np.array(vals, np.float32)
+
+
+def allowed_mask(tokens, vocab):
+    """One row of aotk_logits_rules' masks that allows `tokens` only."""
+    bits = np.zeros((vocab + 31) // 32 * 32, np.uint8)
+    bits[np.asarray(list(tokens), np.int64)] = 1
+    return np.packbits(bits, bitorder="little").view("<u4")
+
+
+def _rules(out_ptr, logits_ptr, kind, rows, vocab, stride, rules, masks, tokens_ptr):
+    table, hist, ids, vals = logits_rules_table(rules)
+    assert len(table) == rows, "one dict of rules per row"
+    masks = np.zeros((0, (vocab + 31) // 32), np.uint32) if masks is None else np.ascontiguousarray(masks, np.uint32)
+    masks = masks.reshape(-1, (vocab + 31) // 32)
+    bufs = [DeviceBuffer.from_numpy(a) if a.size else None for a in (hist, ids, vals, masks)]
+    ptr = [b.ptr if b else None for b in bufs]
+    abi.check(_lib().aotk_logits_rules(out_ptr, logits_ptr, kind, rows, vocab, stride, _np_ptr(table), ptr[0], hist.size,
+                                       ptr[1], ptr[2], ids.size, ptr[3], len(masks), tokens_ptr))
+
+
+def logits_rules(logits, rules, masks=None, kind=abi.F32):
+    """(logits, picks) after each row's rules (aotk_logits_rules); `logits`
+    [rows][vocab], `rules` one dict per row (logits_rules_table), `masks`
+    rows of 32-token words (allowed_mask)."""
+    t = FLOAT_DTYPES[kind]
+    logits = np.ascontiguousarray(logits)
+    rows, vocab = logits.shape
+    dx = _dev(logits, t)
+    out, tok = DeviceBuffer(dx.nbytes), DeviceBuffer(4 * rows)
+    _rules(out.ptr, dx.ptr, kind, rows, vocab, vocab, rules, masks, tok.ptr)
+    return out.to_numpy(t).reshape(rows, vocab), tok.to_numpy(np.uint32)
+
+
 def argmax(x):
     dx = DeviceBuffer.from_numpy(np.asarray(x, np.float32))
     out = C.c_uint32()
@@ -394,6 +496,17 @@ class State:
         x = np.ascontiguousarray(logits, np.float32)
         assert x.size == self.vocab
         abi.check(_lib().aotk_set_logits(self.h, x.ctypes.data_as(C.POINTER(C.c_float))))
+
+    def apply_rules(self, rule, mask=None):
+        """Rules on the current logits, in place, ahead of `sample` or
+        `greedy` (aotk_logits_rules): `rule` a dict (logits_rules_table),
+        `mask` one row of allowed tokens (allowed_mask). Returns the greedy
+        pick, NO_TOKEN where no token is left."""
+        p = abi.check_ptr(_lib().aotk_logits_dev(self.h))
+        tok = DeviceBuffer(4)
+        rule = dict(rule, mask=rule.get("mask", -1 if mask is None else 0))
+        _rules(p, p, abi.F32, 1, self.vocab, self.vocab, [rule], mask, tok.ptr)
+        return int(tok.to_numpy(np.uint32)[0])
 
     def sample(self, sampler, recent=()):
         """Sampler::sample on the current logits (modified in place)."""

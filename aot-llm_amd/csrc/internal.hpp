@@ -258,6 +258,47 @@ size_t attention_scratch_bytes(size_t n_head, size_t head_dim, size_t ctx, size_
 // output. Writes out [n_head * head_dim].
 void launch_attention_decode(float *out, const QkvPost &p, size_t ctx_rows, size_t pos0, size_t window,
                              const int *pos_dev, float *scratch, hipStream_t s);
+// attend.hip: rows over a range that all sequences share, then a range of
+// their own (see there for what a row sees).
+struct AttendSeq {
+    uint32_t row0, rows;  // rows of q and out, packed
+    uint64_t len;         // positions of its own range, its rows the last ones
+    uint64_t cache;       // first of them in the caches, in positions
+};
+constexpr int ATTEND_SEQS = 64;  // sequences whose places travel in one launch's arguments
+struct AttendSeqs {
+    AttendSeq seq[ATTEND_SEQS];
+};
+struct AttendArgs {
+    const void *q;
+    void *out;
+    const void *k_prefix, *v_prefix;  // [n_prefix][kv_dim]
+    const void *k, *v;
+    uint64_t n_prefix, window, n_sink;  // window 0: everything
+    uint32_t n_head, n_kv_head;
+    float scale;
+};
+size_t attend_scratch_bytes(const AttendArgs &a, const AttendSeq *seqs, size_t n);
+void launch_attend(int kind, int head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n, void *scratch, hipStream_t s);
+
+// rules.hip
+constexpr int RULE_SLICE = 4096;  // tokens of one block
+constexpr int RULE_ROWS = 64;     // rows whose rules travel in one launch's arguments
+struct RuleRows {
+    aotk_logits_rule rule[RULE_ROWS];
+};
+struct RuleArgs {
+    void *out;
+    const void *logits;
+    size_t stride;  // elements between rows
+    uint32_t vocab, row0;
+    const uint32_t *hist, *bias_id, *mask;
+    const float *bias;
+    uint64_t *keys;  // rules_scratch_bytes, null: no picks
+};
+size_t rules_scratch_bytes(size_t rows, size_t vocab);
+void launch_rules(int kind, RuleArgs a, const aotk_logits_rule *rules, size_t rows, uint32_t *tokens, hipStream_t s);
+
 void launch_add(float *x, const float *y, size_t n, hipStream_t s);
 void launch_rmsnorm_add(float *x, const float *y, const float *w, size_t n, size_t m, float eps, hipStream_t s);
 // x += rmsnorm(y) * w_post, then rmsnorm(x) * w_next quantized into `out`.

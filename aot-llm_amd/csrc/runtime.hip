@@ -8,6 +8,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <mutex>
 #include <string>
 #include <vector>
 #include <stdlib.h>
@@ -497,6 +498,252 @@ int aotk_attention(float *out_dev, const float *q_dev, const float *k_cache_dev,
     launch_attention(out_dev, q_dev, k_cache_dev + layer * ctx * kv, v_cache_dev + layer * ctx * kv, n_head, n_kv_head,
                      head_dim, ctx, pos0, m, window, (float *)s, g_stream);
     return finish_op();
+}
+
+}  // extern "C"
+
+// The operators for batches of continuations. They share one workspace, grown
+// on demand, and hold its lock until their work on the stream is done, so that
+// several threads may call them; a caller whose current device is another one
+// gets it back.
+static std::mutex g_ops_mutex;
+static void *g_ops_ws = nullptr;
+static size_t g_ops_ws_bytes = 0;
+
+struct DeviceScope {
+    int before = -1;
+    bool ok = false;
+    DeviceScope() {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        ok = before == g_device || hipSetDevice(g_device) == hipSuccess;
+    }
+    ~DeviceScope() {
+        if (before >= 0 && before != g_device) (void)hipSetDevice(before);
+    }
+};
+
+static int ops_workspace(size_t bytes) {
+    if (bytes <= g_ops_ws_bytes) return 0;
+    if (g_ops_ws) (void)hipFree(g_ops_ws);
+    g_ops_ws = nullptr;
+    g_ops_ws_bytes = 0;
+    const size_t want = align_up(bytes, 1 << 20);
+    if (hipMalloc(&g_ops_ws, want) != hipSuccess) {
+        (void)hipGetLastError();
+        g_ops_ws = nullptr;
+        return fail("hipMalloc of %zu workspace bytes failed", want);
+    }
+    g_ops_ws_bytes = want;
+    return 0;
+}
+
+static bool overlaps(const void *a, size_t an, const void *b, size_t bn) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return an && bn && x < y + bn && y < x + an;
+}
+
+// a * b * c * d elements of `size` bytes, false where that passes 63 bits.
+static bool bytes_of(size_t &out, size_t size, size_t a, size_t b, size_t c, size_t d) {
+    unsigned __int128 n = (unsigned __int128)a * b;
+    if (n >> 63) return false;
+    n *= c;
+    if (n >> 63) return false;
+    n *= d;
+    if (n >> 63) return false;
+    n *= size;
+    if (n >> 63) return false;
+    out = (size_t)n;
+    return true;
+}
+
+static int check_kind(const char *what, int kind, const void *const *ptrs, int n) {
+    if (kind != AOTK_F32 && kind != AOTK_F16 && kind != AOTK_BF16) return fail("%s: kind %d is not f32, f16 or bf16", what, kind);
+    for (int i = 0; i < n; i++)
+        if ((uintptr_t)ptrs[i] % type_size(kind)) return fail("%s: a pointer is not aligned to its elements", what);
+    return 0;
+}
+
+static int check_heads(const char *what, size_t n_head, size_t n_kv_head, size_t head_dim) {
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail("%s: head_dim %zu unsupported", what, head_dim);
+    if (n_head == 0 || n_kv_head == 0 || n_head % n_kv_head || n_head > 65535) return fail("%s: bad head counts", what);
+    return 0;
+}
+
+// Rows over all heads that a call may have: they are counted in 31 bits.
+static constexpr size_t ATTEND_MAX_ROWS = size_t(1) << 30;
+
+static int attend(const char *what, int kind, size_t head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n) {
+    if (ops_workspace(attend_scratch_bytes(a, seqs, n))) return -1;
+    launch_attend(kind, (int)head_dim, a, seqs, n, g_ops_ws, g_stream);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
+    if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
+    return 0;
+}
+
+extern "C" {
+
+int aotk_attention_sinks(void *out_dev, const void *q_dev, const void *k_cache_dev, const void *v_cache_dev, int kind,
+                         size_t n_head, size_t n_kv_head, size_t head_dim, size_t ctx, size_t layer, size_t pos0, size_t m,
+                         size_t window, size_t n_sink) {
+    const char *what = "attention_sinks";
+    const void *ptrs[4] = {out_dev, q_dev, k_cache_dev, v_cache_dev};
+    if (check_kind(what, kind, ptrs, 4) || check_heads(what, n_head, n_kv_head, head_dim)) return -1;
+    if (m == 0) return fail("%s: no rows", what);
+    if (m > ctx || pos0 > ctx - m) return fail("%s: positions exceed the context", what);
+    if (!out_dev || !q_dev || !k_cache_dev || !v_cache_dev) return fail("%s: null argument", what);
+    const size_t size = type_size(kind);
+    size_t rows, held, cache;
+    if (m * n_head > ATTEND_MAX_ROWS || m > ATTEND_MAX_ROWS) return fail("%s: %zu rows of %zu heads are too many", what, m, n_head);
+    if (layer > (size_t(1) << 32) || !bytes_of(cache, size, layer + 1, ctx, n_kv_head, head_dim) ||
+        !bytes_of(held, size, pos0 + m, n_kv_head, head_dim, 1) || !bytes_of(rows, size, m, n_head, head_dim, 1))
+        return fail("%s: the cache is too large", what);
+    const size_t first = cache / (layer + 1) * layer;
+    AttendArgs a = {};
+    a.q = q_dev;
+    a.out = out_dev;
+    a.k = (const uint8_t *)k_cache_dev + first;
+    a.v = (const uint8_t *)v_cache_dev + first;
+    if (overlaps(out_dev, rows, q_dev, rows) || overlaps(out_dev, rows, a.k, held) || overlaps(out_dev, rows, a.v, held))
+        return fail("%s: the output overlaps an input", what);
+    // a window that reaches everything is none
+    a.window = window < pos0 + m ? window : 0;
+    a.n_sink = n_sink < pos0 + m ? n_sink : pos0 + m;
+    a.n_head = (uint32_t)n_head;
+    a.n_kv_head = (uint32_t)n_kv_head;
+    a.scale = 1.0f / sqrtf((float)head_dim);
+    const AttendSeq seq = {0, (uint32_t)m, pos0 + m, 0};
+    std::lock_guard<std::mutex> hold(g_ops_mutex);
+    if (ensure_init()) return -1;
+    DeviceScope dev;
+    if (!dev.ok) return fail("%s: the device cannot be selected", what);
+    return attend(what, kind, head_dim, a, &seq, 1);
+}
+
+int aotk_attention_shared(void *out_dev, const void *q_dev, const void *k_prefix_dev, const void *v_prefix_dev,
+                          const void *k_tail_dev, const void *v_tail_dev, int kind, size_t n_head, size_t n_kv_head,
+                          size_t head_dim, size_t prefix_ctx, size_t n_prefix, size_t tail_ctx, size_t layer, size_t batch,
+                          const uint32_t *tail_len_host, const uint32_t *rows_host) {
+    const char *what = "attention_shared";
+    const void *ptrs[6] = {out_dev, q_dev, k_prefix_dev, v_prefix_dev, k_tail_dev, v_tail_dev};
+    if (check_kind(what, kind, ptrs, 6) || check_heads(what, n_head, n_kv_head, head_dim)) return -1;
+    if (batch == 0) return fail("%s: no sequences", what);
+    if (batch > 65535) return fail("%s: %zu sequences, at most 65535", what, batch);
+    if (!tail_len_host) return fail("%s: null argument", what);
+    if (n_prefix > prefix_ctx) return fail("%s: a prefix of %zu positions exceeds its %zu", what, n_prefix, prefix_ctx);
+    size_t total = 0, longest = 0;
+    for (size_t b = 0; b < batch; b++) {
+        if (tail_len_host[b] > tail_ctx) return fail("%s: tail %zu has %u positions, room for %zu", what, b, tail_len_host[b], tail_ctx);
+        total += rows_host ? rows_host[b] : 1;
+        longest = longest > tail_len_host[b] ? longest : tail_len_host[b];
+    }
+    if (total == 0) return 0;
+    if (total * n_head > ATTEND_MAX_ROWS) return fail("%s: %zu rows of %zu heads are too many", what, total, n_head);
+    if (!out_dev || !q_dev || (n_prefix && (!k_prefix_dev || !v_prefix_dev)) || (longest && (!k_tail_dev || !v_tail_dev)))
+        return fail("%s: null argument", what);
+    const size_t size = type_size(kind);
+    size_t rows, prefix, held, tails;
+    if (layer > (size_t(1) << 32) || !bytes_of(prefix, size, layer + 1, prefix_ctx, n_kv_head, head_dim) ||
+        !bytes_of(tails, size * batch, layer + 1, tail_ctx, n_kv_head, head_dim) ||
+        !bytes_of(rows, size, total, n_head, head_dim, 1) || !bytes_of(held, size, n_prefix, n_kv_head, head_dim, 1))
+        return fail("%s: the caches are too large", what);
+    AttendArgs a = {};
+    a.q = q_dev;
+    a.out = out_dev;
+    if (n_prefix) {
+        a.k_prefix = (const uint8_t *)k_prefix_dev + prefix / (layer + 1) * layer;
+        a.v_prefix = (const uint8_t *)v_prefix_dev + prefix / (layer + 1) * layer;
+    }
+    tails /= layer + 1;
+    if (longest) {
+        a.k = (const uint8_t *)k_tail_dev + tails * layer;
+        a.v = (const uint8_t *)v_tail_dev + tails * layer;
+    } else {
+        tails = 0;
+    }
+    if (overlaps(out_dev, rows, q_dev, rows) || overlaps(out_dev, rows, a.k_prefix, held) || overlaps(out_dev, rows, a.v_prefix, held) ||
+        overlaps(out_dev, rows, a.k, tails) || overlaps(out_dev, rows, a.v, tails))
+        return fail("%s: the output overlaps an input", what);
+    a.n_prefix = n_prefix;
+    a.n_head = (uint32_t)n_head;
+    a.n_kv_head = (uint32_t)n_kv_head;
+    a.scale = 1.0f / sqrtf((float)head_dim);
+    AttendSeq *seqs = (AttendSeq *)malloc(batch * sizeof(AttendSeq));
+    if (!seqs) return fail("%s: no memory for %zu sequences", what, batch);
+    uint32_t row0 = 0;
+    for (size_t b = 0; b < batch; b++) {
+        const uint32_t r = rows_host ? rows_host[b] : 1;
+        seqs[b] = {row0, r, tail_len_host[b], b * tail_ctx};
+        row0 += r;
+    }
+    int rc = -1;
+    {
+        std::lock_guard<std::mutex> hold(g_ops_mutex);
+        if (!ensure_init()) {
+            DeviceScope dev;
+            rc = dev.ok ? attend(what, kind, head_dim, a, seqs, batch) : fail("%s: the device cannot be selected", what);
+        }
+    }
+    free(seqs);
+    return rc;
+}
+
+int aotk_logits_rules(void *out_dev, const void *logits_dev, int kind, size_t rows, size_t vocab, size_t stride,
+                      const aotk_logits_rule *rules_host, const uint32_t *hist_dev, size_t n_hist,
+                      const uint32_t *bias_id_dev, const float *bias_dev, size_t n_bias, const uint32_t *mask_dev,
+                      size_t n_mask, uint32_t *tokens_dev) {
+    const char *what = "logits_rules";
+    const void *ptrs[2] = {out_dev, logits_dev};
+    if (check_kind(what, kind, ptrs, 2)) return -1;
+    for (const void *p : {(const void *)hist_dev, (const void *)bias_id_dev, (const void *)bias_dev, (const void *)mask_dev, (const void *)tokens_dev})
+        if ((uintptr_t)p % 4) return fail("%s: a pointer is not aligned to its elements", what);
+    if (rows == 0 || vocab == 0) return fail("%s: no logits", what);
+    if (vocab > 0x7fffffffu || rows > 0x7fffffffu) return fail("%s: %zu rows of %zu logits are too many", what, rows, vocab);
+    if (stride < vocab) return fail("%s: rows of %zu logits overlap at a stride of %zu", what, vocab, stride);
+    if (!out_dev || !logits_dev || !rules_host) return fail("%s: null argument", what);
+    for (size_t i = 0; i < rows; i++) {
+        const aotk_logits_rule &r = rules_host[i];
+        if (!(r.repetition > 0.0f) || isinf(r.repetition)) return fail("%s: row %zu: a repetition penalty of %g", what, i, (double)r.repetition);
+        if (!isfinite(r.presence) || !isfinite(r.frequency)) return fail("%s: row %zu: a penalty is not finite", what, i);
+        if ((uint64_t)r.hist_off + r.hist_len > n_hist) return fail("%s: row %zu: history outside the %zu tokens", what, i, n_hist);
+        if ((uint64_t)r.bias_off + r.bias_len > n_bias) return fail("%s: row %zu: biases outside the %zu entries", what, i, n_bias);
+        if (r.mask < -1 || (r.mask >= 0 && (size_t)r.mask >= n_mask)) return fail("%s: row %zu: mask %d of %zu", what, i, r.mask, n_mask);
+        if ((r.hist_len && !hist_dev) || (r.bias_len && (!bias_id_dev || !bias_dev)) || (r.mask >= 0 && !mask_dev))
+            return fail("%s: null argument", what);
+    }
+    const size_t size = type_size(kind);
+    size_t bytes, masks, picks;
+    if (!bytes_of(bytes, size, rows, stride, 1, 1) || !bytes_of(masks, 4, n_mask, (vocab + 31) / 32, 1, 1) ||
+        !bytes_of(picks, 4, rows, 1, 1, 1) || n_hist > (size_t(1) << 60) || n_bias > (size_t(1) << 60))
+        return fail("%s: the tensors are too large", what);
+    bytes -= (stride - vocab) * size;  // the last row ends with its logits
+    const struct { const void *p; size_t n; } in[4] = {{hist_dev, n_hist * 4}, {bias_id_dev, n_bias * 4}, {bias_dev, n_bias * 4}, {mask_dev, masks}};
+    for (const auto &x : in)
+        if (x.p && (overlaps(out_dev, bytes, x.p, x.n) || (tokens_dev && overlaps(tokens_dev, picks, x.p, x.n))))
+            return fail("%s: an output overlaps an input", what);
+    if ((out_dev != logits_dev && overlaps(out_dev, bytes, logits_dev, bytes)) ||
+        (tokens_dev && (overlaps(tokens_dev, picks, logits_dev, bytes) || overlaps(tokens_dev, picks, out_dev, bytes))))
+        return fail("%s: an output overlaps an input", what);
+    std::lock_guard<std::mutex> hold(g_ops_mutex);
+    if (ensure_init()) return -1;
+    DeviceScope dev;
+    if (!dev.ok) return fail("%s: the device cannot be selected", what);
+    if (tokens_dev && ops_workspace(rules_scratch_bytes(rows, vocab))) return -1;
+    RuleArgs a = {};
+    a.out = out_dev;
+    a.logits = logits_dev;
+    a.stride = stride;
+    a.vocab = (uint32_t)vocab;
+    a.hist = hist_dev;
+    a.bias_id = bias_id_dev;
+    a.bias = bias_dev;
+    a.mask = mask_dev;
+    a.keys = tokens_dev ? (uint64_t *)g_ops_ws : nullptr;
+    launch_rules(kind, a, rules_host, rows, tokens_dev, g_stream);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
+    if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
+    return 0;
 }
 
 int aotk_argmax(const float *x_dev, size_t n, uint32_t *out_host) {
@@ -1177,6 +1424,14 @@ int aotk_logits(aotk_state *st, float *out_host) {
     HIPC(hipMemcpyAsync(out_host, st->logits, st->m->spec.dims.vocab * 4, hipMemcpyDeviceToHost, g_stream));
     HIPC(hipStreamSynchronize(g_stream));
     return 0;
+}
+
+float *aotk_logits_dev(aotk_state *st) {
+    if (!st) {
+        fail("null state");
+        return nullptr;
+    }
+    return st->logits;
 }
 
 int aotk_greedy(aotk_state *st, uint32_t *token_out) {

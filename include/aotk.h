@@ -244,6 +244,74 @@ int aotk_add(float *x_dev, const float *y_dev, size_t n);
 int aotk_attention(float *out_dev, const float *q_dev, const float *k_cache_dev, const float *v_cache_dev,
                    size_t n_head, size_t n_kv_head, size_t head_dim, size_t ctx, size_t layer,
                    size_t pos0, size_t m, size_t window);
+
+/* The operators below serve many continuations of one prefix. They have no
+ * counterpart in the reference. Their element kind is AOTK_F32, AOTK_F16 or
+ * AOTK_BF16, the same for all tensors of a call; scores, softmax statistics
+ * and sums are f32, and results are rounded once to the kind, to nearest.
+ * Pointers need the alignment of one element. Outputs must not overlap inputs
+ * (aotk_logits_rules may write its logits in place). They may be called from
+ * several host threads at once. */
+
+/* Attention of m rows at positions pos0..pos0+m-1 over a
+ * [n_layer][ctx][kv_dim] cache, like aotk_attention, where the row at
+ * position p sees the positions j <= p with j > p - window (the sliding
+ * window) or j < n_sink (the first positions stay visible). window 0 = every
+ * position. Any number of query heads per kv head, any context length. What
+ * the cache holds at positions that a row does not see, infinities and NaN
+ * included, does not reach the row.
+ * q_dev, out_dev: [m][n_head][head_dim]; head_dim 64, 128 or 256. */
+int aotk_attention_sinks(void *out_dev, const void *q_dev, const void *k_cache_dev, const void *v_cache_dev, int kind,
+                         size_t n_head, size_t n_kv_head, size_t head_dim, size_t ctx, size_t layer, size_t pos0,
+                         size_t m, size_t window, size_t n_sink);
+
+/* Attention of a batch of sequences that share a prefix, whose keys and
+ * values are read once for all of them.
+ *   k_prefix_dev, v_prefix_dev: [n_layer][prefix_ctx][kv_dim], the first
+ *     n_prefix positions hold the prefix (e.g. a state's cache after
+ *     aotk_prefix_load);
+ *   k_tail_dev, v_tail_dev: [n_layer][batch][tail_ctx][kv_dim], sequence b
+ *     holds tail_len_host[b] <= tail_ctx positions of its own;
+ *   rows_host[b] rows of sequence b (null: one each, the decode step), packed
+ *     in q_dev and out_dev [sum of rows][n_head][head_dim] without gaps. They
+ *     are the newest of its positions: row i sees the whole prefix and the
+ *     tail positions j <= tail_len_host[b] - rows_host[b] + i (none where
+ *     that is negative).
+ * A row that sees nothing at all is 0. Sequences without rows are skipped.
+ * The two _host arrays have `batch` entries. */
+int aotk_attention_shared(void *out_dev, const void *q_dev, const void *k_prefix_dev, const void *v_prefix_dev,
+                          const void *k_tail_dev, const void *v_tail_dev, int kind, size_t n_head, size_t n_kv_head,
+                          size_t head_dim, size_t prefix_ctx, size_t n_prefix, size_t tail_ctx, size_t layer,
+                          size_t batch, const uint32_t *tail_len_host, const uint32_t *rows_host);
+
+/* The rules of one row of logits (aotk_logits_rules). */
+typedef struct aotk_logits_rule {
+    float repetition;  /* > 0, 1 = none */
+    float presence;    /* 0 = none */
+    float frequency;   /* 0 = none */
+    uint32_t hist_off, hist_len; /* the row's tokens so far: hist_dev[hist_off ..+ hist_len) */
+    uint32_t bias_off, bias_len; /* its biases: entries [bias_off ..+ bias_len) */
+    int32_t mask;      /* row of mask_dev, -1 = every token is allowed */
+} aotk_logits_rule;
+
+/* Rules on a batch of logits, [rows][stride] of which `vocab` values a row
+ * are read and written, out_dev == logits_dev or apart. For each token t, c =
+ * how often it occurs in the row's history:
+ *   c > 0: x = (x > 0 ? x / repetition : x * repetition) - (presence + frequency * c)
+ *   x += the bias of the last entry whose id is t
+ *   a mask is given and bit t % 32 of its word t / 32 is 0: x = -inf
+ * (unlike aotk_sampler's repeat_penalty, the repetition penalty applies once
+ * however often a token occurs). mask_dev: n_mask rows of (vocab + 31) / 32
+ * words, which rows of logits may share. History tokens and bias ids >= vocab
+ * name nothing.
+ * tokens_dev (may be null): each row's greedy pick, the first index of the
+ * largest value written (NaN is passed over), 0xFFFFFFFF where nothing above
+ * -inf is left. rules_host has `rows` entries. */
+int aotk_logits_rules(void *out_dev, const void *logits_dev, int kind, size_t rows, size_t vocab, size_t stride,
+                      const aotk_logits_rule *rules_host, const uint32_t *hist_dev, size_t n_hist,
+                      const uint32_t *bias_id_dev, const float *bias_dev, size_t n_bias, const uint32_t *mask_dev,
+                      size_t n_mask, uint32_t *tokens_dev);
+
 /* First index of the strict maximum: sampler.rs:99-109. */
 int aotk_argmax(const float *x_dev, size_t n, uint32_t *out_host);
 
@@ -319,6 +387,9 @@ int aotk_sampler_free(aotk_sampler *sampler);
  * repetition penalty, sampler.rs:53-60), `recent` = the tokens so far
  * (the last repeat_last_n are penalised). */
 int aotk_sample(aotk_state *state, aotk_sampler *sampler, const uint32_t *recent, size_t n_recent, uint32_t *token_out);
+/* The state's vocab logits in device memory, f32 (for aotk_logits_rules
+ * between a forward and aotk_sample or aotk_greedy). */
+float *aotk_logits_dev(aotk_state *state);
 /* Replace the state's vocab logits (the `logits: &mut [f32]` argument of
  * Sampler::sample, sampler.rs:49) with a host array. */
 int aotk_set_logits(aotk_state *state, const float *logits_host);
