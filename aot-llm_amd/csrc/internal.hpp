@@ -265,10 +265,6 @@ struct AttendSeq {
     uint64_t len;         // positions of its own range, its rows the last ones
     uint64_t cache;       // first of them in the caches, in positions
 };
-constexpr int ATTEND_SEQS = 64;  // sequences whose places travel in one launch's arguments
-struct AttendSeqs {
-    AttendSeq seq[ATTEND_SEQS];
-};
 struct AttendArgs {
     const void *q;
     void *out;
@@ -278,7 +274,44 @@ struct AttendArgs {
     uint32_t n_head, n_kv_head;
     float scale;
 };
-size_t attend_scratch_bytes(const AttendArgs &a, const AttendSeq *seqs, size_t n);
+// The keys that rows at positions pmin..pmax see between them: na keys of
+// range A (the prefix's, or the sequence's first), then own positions b0.. of
+// which nb. Given `prefix` keys in A, or none, and then the sinks are there if
+// they lie apart from the window.
+struct AttendSpan {
+    uint64_t na, b0, nb;
+};
+__host__ __device__ inline AttendSpan attend_span(uint64_t prefix, uint64_t window, uint64_t n_sink, int64_t pmin, int64_t pmax) {
+    const int64_t lo = window && pmin >= (int64_t)window ? pmin - (int64_t)window + 1 : 0;
+    AttendSpan s = {prefix, 0, pmax >= 0 ? (uint64_t)pmax + 1 : 0};
+    if (lo > (int64_t)n_sink) {  // the window has left the sinks behind
+        if (!prefix) s.na = n_sink;
+        s.b0 = (uint64_t)lo;
+        s.nb -= (uint64_t)lo;
+    }
+    return s;
+}
+constexpr int ATTEND_SEQS = 64;  // sequences whose places travel in one launch's arguments
+struct AttendPlace {
+    uint32_t row0, rows;
+    uint64_t len, cache;
+    uint32_t block0, chunks;  // first block of the launch, runs of its key tiles
+    uint64_t part0;           // first partial result, in rows
+};
+struct AttendLaunch {
+    const void *q;
+    void *out;
+    const void *ka, *va, *k, *v;
+    float *part_ml, *part_acc;
+    uint64_t na, window, n_sink;
+    uint32_t n_head, n_kv_head, n_seq, run;
+    float scale_log2;
+    uint32_t causal;   // 0: every row sees all `len` positions
+    uint32_t sinks_a;  // range A is the sequence's own cache
+    uint32_t joined;   // every row has partial results elsewhere too
+    AttendPlace seq[ATTEND_SEQS];
+};
+size_t attend_scratch_bytes(int kind, int head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n);
 void launch_attend(int kind, int head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n, void *scratch, hipStream_t s);
 
 // rules.hip

@@ -565,7 +565,8 @@ static int check_kind(const char *what, int kind, const void *const *ptrs, int n
 
 static int check_heads(const char *what, size_t n_head, size_t n_kv_head, size_t head_dim) {
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail("%s: head_dim %zu unsupported", what, head_dim);
-    if (n_head == 0 || n_kv_head == 0 || n_head % n_kv_head || n_head > 65535) return fail("%s: bad head counts", what);
+    // (the kernels' offsets inside a tile of keys are 32 bits)
+    if (n_head == 0 || n_kv_head == 0 || n_head % n_kv_head || n_head > 16384) return fail("%s: bad head counts", what);
     return 0;
 }
 
@@ -573,7 +574,7 @@ static int check_heads(const char *what, size_t n_head, size_t n_kv_head, size_t
 static constexpr size_t ATTEND_MAX_ROWS = size_t(1) << 30;
 
 static int attend(const char *what, int kind, size_t head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n) {
-    if (ops_workspace(attend_scratch_bytes(a, seqs, n))) return -1;
+    if (ops_workspace(attend_scratch_bytes(kind, (int)head_dim, a, seqs, n))) return -1;
     launch_attend(kind, (int)head_dim, a, seqs, n, g_ops_ws, g_stream);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) e = hipStreamSynchronize(g_stream);

@@ -27,7 +27,7 @@ SINKS = dict(out=OUT, q=Q, k=K, v=V, kind=0, n_head=8, n_kv_head=2, head_dim=64,
 
 @pytest.mark.parametrize("change,what", [
     (dict(kind=5), "kind 5"), (dict(kind=-1), "kind -1"), (dict(head_dim=80), "head_dim 80"), (dict(n_head=0), "head counts"),
-    (dict(n_kv_head=0), "head counts"), (dict(n_kv_head=3), "head counts"), (dict(n_head=65536 * 2), "head counts"),
+    (dict(n_kv_head=0), "head counts"), (dict(n_kv_head=3), "head counts"), (dict(n_head=16386), "head counts"),
     (dict(m=0), "no rows"), (dict(pos0=96), "exceed the context"), (dict(pos0=2 ** 64 - 3), "exceed the context"),
     (dict(m=101, pos0=0), "exceed the context"), (dict(out=None), "null"), (dict(q=None), "null"), (dict(k=None), "null"),
     (dict(v=None), "null"), (dict(q=Q + 2), "aligned"), (dict(out=Q), "overlaps"), (dict(out=K + 64), "overlaps"),
