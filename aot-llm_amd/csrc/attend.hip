@@ -22,6 +22,8 @@
 // positions, heads fastest) and a run of key tiles. Where runs are cut or a
 // prefix is joined to tails, blocks leave (maximum, sum, accumulator) in f32
 // and k_join puts them together.
+#include <math.h>
+
 #include "device.hpp"
 #include "internal.hpp"
 
@@ -291,15 +293,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : (RB == 2 ? 2 : 3)) void k_atten
 #pragma unroll
             for (int h = 0; h < NK / 16; h++) {
                 sc[b][h] = f32x4{0, 0, 0, 0};
+                if constexpr (F32) {  // four chains: shorter sums round less
+                    f32x4 part[4];
 #pragma unroll
-                for (int u = 0; u < S::QR; u++) {
-                    if constexpr (F32) {
+                    for (int c = 0; c < 4; c++) {
+                        part[c] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                        for (int c = 0; c < 4; c++)
-                            sc[b][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[h * S::QR + u][c]), __uint_as_float(q[b][u][c]), sc[b][h], 0, 0, 0);
-                    } else {
-                        sc[b][h] = AttElem<KIND>::mma16(k[h * S::QR + u], q[b][u], sc[b][h]);
+                        for (int u = 0; u < S::QR; u++)
+                            part[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[h * S::QR + u][c]), __uint_as_float(q[b][u][c]), part[c], 0, 0, 0);
                     }
+                    sc[b][h] = (part[0] + part[1]) + (part[2] + part[3]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < S::QR; u++) sc[b][h] = AttElem<KIND>::mma16(k[h * S::QR + u], q[b][u], sc[b][h]);
                 }
             }
         if (more) load_k(nx);
@@ -749,20 +755,23 @@ __global__ __launch_bounds__(NW * 64) void k_attend_wide(AttendLaunch a) {
 }
 
 // ------------------------------------------------------------------- join
-// One wave per row and query head: the runs of the prefix, then those of the
-// sequence's own range.
-template <int KIND, int D>
+// WAVES waves per row and query head: the runs of the prefix, then those of the
+// sequence's own range. A lane holds the weight of every 64th run; each wave
+// sums every WAVES-th run's accumulators, four loads in flight.
+template <int KIND, int D, int WAVES>
 __global__ __launch_bounds__(256) void k_join(AttendLaunch a, uint32_t prefix_chunks, uint32_t total, uint32_t row_begin) {
     constexpr int N = D / 64;
-    const int lane = threadIdx.x & 63;
-    const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6);
+    typedef float vec __attribute__((ext_vector_type(N)));
+    __shared__ float l_acc[4][D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % WAVES;
+    const uint32_t item = blockIdx.x * (4 / WAVES) + wave / WAVES;
     const uint32_t row = row_begin + item / a.n_head, head = item % a.n_head;
     const bool le = lane < (int)a.n_seq && a.seq[lane].row0 <= row;
     const uint32_t si = (uint32_t)__builtin_amdgcn_readfirstlane(__popcll(__ballot(le)) - 1);
     const AttendPlace s = a.seq[si];
     const uint32_t i = row - s.row0;
-    if (i >= s.rows || (s.chunks == 1 && !a.joined)) return;
-    const uint32_t n = prefix_chunks + s.chunks;
+    const bool mine = i < s.rows && (s.chunks > 1 || a.joined);
+    const uint32_t n = mine ? prefix_chunks + s.chunks : 0;
     auto slot = [&](uint32_t c) {
         return (c < prefix_chunks ? (size_t)c * total + row : s.part0 + (size_t)(c - prefix_chunks) * s.rows + i) * a.n_head + head;
     };
@@ -771,24 +780,47 @@ __global__ __launch_bounds__(256) void k_join(AttendLaunch a, uint32_t prefix_ch
     for (uint32_t c = lane; c < n; c += 64) mx = fmaxf(mx, ml[slot(c)].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, shfl_xor(mx, o));
-    float acc[N], sum = 0.0f;
+    vec acc = 0.0f;
+    float sum = 0.0f;
+    for (uint32_t c0 = 0; c0 < n; c0 += 64) {
+        float w = 0.0f;
+        if (c0 + lane < n) {
+            const float2 x = ml[slot(c0 + lane)];
+            w = att_shift(x.x, mx);
+            sum += x.y * w;
+        }
+        const uint32_t nc = min(n - c0, 64u);
+        for (uint32_t c = part; c < nc; c += 4 * WAVES) {
+            vec y[4];
+            float f[4];
 #pragma unroll
-    for (int e = 0; e < N; e++) acc[e] = 0.0f;
-    for (uint32_t c = 0; c < n; c++) {
-        const size_t at = slot(c);
-        const float2 x = ml[at];
-        const float f = att_shift(x.x, mx);
-        sum += x.y * f;
+            for (int e = 0; e < 4; e++) {
+                const uint32_t ce = min(c + e * WAVES, nc - 1);
+                y[e] = *(const vec *)(a.part_acc + slot(c0 + ce) * D + lane * N);
+                f[e] = c + e * WAVES < nc ? readlane_f(w, ce) : 0.0f;
+            }
 #pragma unroll
-        for (int e = 0; e < N; e++) acc[e] += a.part_acc[at * D + e * 64 + lane] * f;
+            for (int e = 0; e < 4; e++)
+                if (c + e * WAVES < nc) acc += y[e] * f[e];
+        }
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += shfl_xor(sum, o);
+    if constexpr (WAVES > 1) {
+        *(vec *)&l_acc[wave][lane * N] = acc;
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int e = 1; e < WAVES; e++) acc += *(const vec *)&l_acc[wave + e][lane * N];
+    }
+    if (!mine) return;
     const int64_t p = (int64_t)s.len - s.rows + i;
     const float r = prefix_chunks > 0 || a.na > 0 || p >= 0 ? 1.0f / sum : 0.0f;
+    const size_t at = ((size_t)row * a.n_head + head) * D + lane * N;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-        const size_t at = ((size_t)row * a.n_head + head) * D + e * 64 + lane;
-        if constexpr (KIND == AOTK_F32) ((float *)a.out)[at] = acc[e] * r;
-        else ((uint16_t *)a.out)[at] = (uint16_t)AttElem<KIND>::pair(acc[e] * r, 0.0f);
+        if constexpr (KIND == AOTK_F32) ((float *)a.out)[at + e] = acc[e] * r;
+        else ((uint16_t *)a.out)[at + e] = (uint16_t)AttElem<KIND>::pair(acc[e] * r, 0.0f);
     }
 }
 
@@ -835,12 +867,25 @@ static AttPlan att_plan(int kind, int head_dim, const AttendArgs &a, uint64_t na
     }
     tiles *= a.n_kv_head;
     items *= a.n_kv_head;
-    // enough blocks to fill the chip, none with less than a few tiles
+    if (!items) {
+        p.run = 1;
+        return p;
+    }
+    // As many runs as fill the chip, unless writing and joining their results
+    // (f32, for every row) would cost more than the tiles of a run: c runs of
+    // T tiles take T / c tile times and c times the traffic of one result.
     const bool narrow = p.rows_tile <= 32;
-    const uint64_t want = narrow ? 1024 : 512, least = narrow ? 8 : 4;
-    uint64_t run = items >= want ? tiles : (tiles + want - 1) / want;
-    if (run < least) run = least;
-    p.run = (uint32_t)(run < 0x7fffffffu ? run : 0x7fffffffu);
+    const double want = narrow ? 1024 : 512, least = narrow ? 4 : 1;
+    double cuts = want / (double)items;
+    if (!narrow) {
+        const double tile_us = 4.0 * p.rows_tile * p.nk * head_dim / (kind == AOTK_F32 ? 0.5e6 : 3.5e6);
+        const double part_us = (double)items * p.rows_tile * head_dim * 8 / 4e6;
+        const double most_cuts = sqrt((double)tiles / (double)items * tile_us / part_us);
+        cuts = cuts < most_cuts ? cuts : most_cuts;
+    }
+    if (cuts < 1) cuts = 1;
+    const double run = ceil((double)tiles / (double)items / floor(cuts));
+    p.run = items >= want ? 0x7fffffffu : (uint32_t)(run > least ? run : least);
     return p;
 }
 
@@ -849,7 +894,7 @@ static uint32_t att_chunks(const AttendArgs &a, uint64_t na, bool causal, const 
     const uint32_t rt = att_row_tiles(s.rows, group, p.rows_tile);
     // spans grow with the position until the window is full: the last tile's is the longest, or within a tile of it
     uint64_t t = att_tiles(a, na, causal, s, group, p, rt - 1);
-    if (rt > 1) {
+    if (causal && rt > 1) {
         const uint64_t u = att_tiles(a, na, causal, s, group, p, rt - 2);
         t = t > u ? t : u;
         t += 2;
@@ -956,13 +1001,14 @@ static void attend_all(const AttendArgs &a, const AttendSeq *seqs, size_t n, voi
     uint64_t part = (uint64_t)w.prefix_chunks * w.total;
     const uint64_t na = l.na;
     for (size_t b0 = 0; b0 < n; b0 += ATTEND_SEQS) {
-        uint32_t blocks = 0, first_row = 0, last_row = 0;
+        uint32_t blocks = 0, first_row = 0, last_row = 0, most = 0;
         bool parts = false;
         l.n_seq = 0;
         for (size_t b = b0; b < n && b < b0 + ATTEND_SEQS; b++) {
             const AttendSeq &q = seqs[b];
             if (!q.rows) continue;
             const uint32_t c = att_chunks(a, na, true, q, w.group, w.own);
+            most = most > c ? most : c;
             if (l.n_seq == 0) first_row = q.row0;
             last_row = q.row0 + q.rows;
             l.seq[l.n_seq++] = {q.row0, q.rows, q.len, q.cache, blocks, c, part};
@@ -976,7 +1022,8 @@ static void attend_all(const AttendArgs &a, const AttendSeq *seqs, size_t n, voi
         att_launch<KIND, D>(w.own, l, blocks, s);
         if (parts) {
             const uint64_t items = (uint64_t)(last_row - first_row) * a.n_head;
-            k_join<KIND, D><<<(unsigned)((items + 3) / 4), 256, 0, s>>>(l, w.prefix_chunks, w.total, first_row);
+            if (w.prefix_chunks + most >= 8) k_join<KIND, D, 4><<<(unsigned)items, 256, 0, s>>>(l, w.prefix_chunks, w.total, first_row);
+            else k_join<KIND, D, 1><<<(unsigned)((items + 3) / 4), 256, 0, s>>>(l, w.prefix_chunks, w.total, first_row);
         }
     }
 }

@@ -316,7 +316,7 @@ void launch_attend(int kind, int head_dim, const AttendArgs &a, const AttendSeq 
 
 // rules.hip
 constexpr int RULE_SLICE = 4096;  // tokens of one block
-constexpr int RULE_ROWS = 64;     // rows whose rules travel in one launch's arguments
+constexpr int RULE_ROWS = 96;    // rows whose rules travel in one launch's arguments
 struct RuleRows {
     aotk_logits_rule rule[RULE_ROWS];
 };
@@ -325,6 +325,7 @@ struct RuleArgs {
     const void *logits;
     size_t stride;  // elements between rows
     uint32_t vocab, row0;
+    uint32_t tables;  // set by launch_rules
     const uint32_t *hist, *bias_id, *mask;
     const float *bias;
     uint64_t *keys;  // rules_scratch_bytes, null: no picks

@@ -21,8 +21,10 @@
 
 namespace aotk {
 
-constexpr int RULE_THREADS = 256;
+constexpr int RULE_THREADS = 512;
 constexpr int RULE_PER = RULE_SLICE / RULE_THREADS;  // values per thread
+
+typedef uint32_t u32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // Rows start at any multiple of the element size: vector accesses that
 // promise no more alignment than that.
@@ -58,7 +60,6 @@ struct RuleVec<AOTK_BF16> {
 // in the low one (the maximum is the largest value's lowest token). 0 stands
 // for no token: NaN and -inf are never picked. Zeros of both signs are equal.
 __device__ __forceinline__ uint64_t rule_key(float y, uint32_t t) {
-    if (!(y > -__builtin_inff())) return 0;
     const uint32_t b = __float_as_uint(y + 0.0f);
     const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
     return ((uint64_t)o << 32) | (uint32_t)~t;
@@ -73,14 +74,45 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
     return k;
 }
 
+// f(token of the slice, place in the list) for the entries of a list of n that
+// name the block's slice. `first` holds the thread's first four.
+template <typename F>
+__device__ __forceinline__ void rule_list(const uint32_t *list, uint32_t n, uint32_t base, u32x4a4 first, F f) {
+    for (uint32_t i = threadIdx.x * 4; i < n; i += RULE_THREADS * 4) {
+        if (i >= RULE_THREADS * 4) {
+            if (i + 4 <= n) first = *(const u32x4a4 *)(list + i);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++) first[e] = i + e < n ? list[i + e] : 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t t = first[e] - base;
+            if (i + e < n && t < (uint32_t)RULE_SLICE) f(t, i + e);
+        }
+    }
+}
+__device__ __forceinline__ u32x4a4 rule_first(const uint32_t *list, uint32_t n) {
+    const uint32_t i = threadIdx.x * 4;
+    u32x4a4 x = {0, 0, 0, 0};
+    if (i + 4 <= n) x = *(const u32x4a4 *)(list + i);
+    else
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (i + e < n) x[e] = list[i + e];
+    return x;
+}
+
+// Everything that a block reads is requested before the first wait: logits,
+// mask words, the heads of the lists. `tables`: what the launch's rows need,
+// 1 a count per token, 2 a bias per token (16 KB of LDS each).
 template <int KIND>
 __global__ __launch_bounds__(RULE_THREADS) void k_rules(RuleArgs a, RuleRows rr) {
     typedef RuleVec<KIND> VT;
     typedef typename VT::elem elem;
     typedef typename VT::vec vec;
     constexpr int N = VT::N, G = RULE_PER / N;
-    __shared__ uint32_t cnt[RULE_SLICE];
-    __shared__ uint32_t last[RULE_SLICE];
+    extern __shared__ __align__(16) uint32_t tables[];
     __shared__ uint64_t best[RULE_THREADS / 64];
     const aotk_logits_rule r = rr.rule[blockIdx.y];
     const size_t row = (size_t)a.row0 + blockIdx.y;
@@ -89,9 +121,13 @@ __global__ __launch_bounds__(RULE_THREADS) void k_rules(RuleArgs a, RuleRows rr)
     const uint32_t left = a.vocab - base;  // tokens of the row from this slice on
     const elem *src = (const elem *)a.logits + row * a.stride + base;
     elem *dst = (elem *)a.out + row * a.stride + base;
+    uint32_t *const cnt = tables, *const last = tables + (a.tables & 1 ? RULE_SLICE : 0);
+    const bool pen = r.hist_len > 0 && (r.repetition != 1.0f || r.presence != 0.0f || r.frequency != 0.0f);
+    const bool biased = r.bias_len > 0;
 
-    // the slice's logits, in flight while the lists are scanned
     vec x[G];
+    uint32_t word[G];
+    const uint32_t *mask = r.mask >= 0 ? a.mask + (size_t)r.mask * ((a.vocab + 31) / 32) + base / 32 : nullptr;
 #pragma unroll
     for (int g = 0; g < G; g++) {
         const uint32_t t = (g * RULE_THREADS + tid) * N;
@@ -99,53 +135,62 @@ __global__ __launch_bounds__(RULE_THREADS) void k_rules(RuleArgs a, RuleRows rr)
         else
 #pragma unroll
             for (int i = 0; i < N; i++) x[g][i] = t + i < left ? src[t + i] : (elem)0;
+        word[g] = mask && t < left ? mask[t / 32] : ~0u;
     }
+    const u32x4a4 h0 = pen ? rule_first(a.hist + r.hist_off, r.hist_len) : u32x4a4{0, 0, 0, 0};
+    const u32x4a4 b0 = biased ? rule_first(a.bias_id + r.bias_off, r.bias_len) : u32x4a4{0, 0, 0, 0};
 
-    const bool pen = r.hist_len > 0 && (r.repetition != 1.0f || r.presence != 0.0f || r.frequency != 0.0f);
-    const bool biased = r.bias_len > 0;
     if (pen || biased) {
-        for (int i = tid; i < RULE_SLICE; i += RULE_THREADS) {
-            cnt[i] = 0;
-            last[i] = 0;
+        const u32x4a4 zero = {0, 0, 0, 0};
+        for (int i = tid * 4; i < RULE_SLICE; i += RULE_THREADS * 4) {
+            if (pen) *(u32x4a4 *)(cnt + i) = zero;
+            if (biased) *(u32x4a4 *)(last + i) = zero;
         }
         __syncthreads();
-        if (pen)
-            for (uint32_t i = tid; i < r.hist_len; i += RULE_THREADS) {
-                const uint32_t t = a.hist[(size_t)r.hist_off + i] - base;
-                if (t < (uint32_t)RULE_SLICE) atomicAdd(&cnt[t], 1u);
-            }
-        if (biased)
-            for (uint32_t i = tid; i < r.bias_len; i += RULE_THREADS) {
-                const uint32_t t = a.bias_id[(size_t)r.bias_off + i] - base;
-                if (t < (uint32_t)RULE_SLICE) atomicMax(&last[t], i + 1);
-            }
+        if (pen) rule_list(a.hist + r.hist_off, r.hist_len, base, h0, [&](uint32_t t, uint32_t) { atomicAdd(&cnt[t], 1u); });
+        if (biased) rule_list(a.bias_id + r.bias_off, r.bias_len, base, b0, [&](uint32_t t, uint32_t i) { atomicMax(&last[t], i + 1); });
         __syncthreads();
     }
-    const uint32_t *mask = r.mask >= 0 ? a.mask + (size_t)r.mask * ((a.vocab + 31) / 32) + base / 32 : nullptr;
 
-    uint64_t key = 0;
+    float top = -__builtin_inff();
+    uint32_t at = 0;
 #pragma unroll
     for (int g = 0; g < G; g++) {
         const uint32_t t = (g * RULE_THREADS + tid) * N;
         if (t >= left) continue;
-        const uint32_t word = mask ? mask[t / 32] >> (t % 32) : ~0u;
-        vec y;
+        const uint32_t bits = word[g] >> (t % 32);
+        vec y = x[g];
+        if (pen || biased) {
+            float v[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            float v = VT::up(x[g][i]);
-            if (pen) {
-                const uint32_t c = cnt[t + i];
-                if (c) v = (v > 0.0f ? v / r.repetition : v * r.repetition) - (r.presence + r.frequency * (float)c);
-            }
-            if (biased) {
-                const uint32_t e = last[t + i];
-                if (e) v = v + a.bias[(size_t)r.bias_off + e - 1];
-            }
-            if (!((word >> i) & 1u)) v = -__builtin_inff();
-            y[i] = VT::down(v);
-            const uint64_t k = t + i < left ? rule_key(VT::up(y[i]), base + t + i) : 0;
-            key = k > key ? k : key;
+            for (int i = 0; i < N; i++) v[i] = VT::up(x[g][i]);
+            if (pen)
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const uint32_t c = cnt[t + i];
+                    if (c) v[i] = (v[i] > 0.0f ? v[i] / r.repetition : v[i] * r.repetition) - (r.presence + r.frequency * (float)c);
+                }
+            if (biased)
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const uint32_t e = last[t + i];
+                    if (e) v[i] = v[i] + a.bias[(size_t)r.bias_off + e - 1];
+                }
+#pragma unroll
+            for (int i = 0; i < N; i++) y[i] = VT::down(v[i]);
         }
+        const elem none = VT::down(-__builtin_inff());
+#pragma unroll
+        for (int i = 0; i < N; i++) y[i] = (bits >> i) & 1u ? y[i] : none;
+        if (a.keys)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float v = VT::up(y[i]);
+                if (v > top && t + i < left) {
+                    top = v;
+                    at = t + i;
+                }
+            }
         if (t + N <= left) *(vec *)(dst + t) = y;
         else
 #pragma unroll
@@ -153,7 +198,7 @@ __global__ __launch_bounds__(RULE_THREADS) void k_rules(RuleArgs a, RuleRows rr)
                 if (t + i < left) dst[t + i] = y[i];
     }
     if (!a.keys) return;
-    key = wave_max_key(key);
+    uint64_t key = wave_max_key(top > -__builtin_inff() ? rule_key(top, base + at) : 0);
     if ((tid & 63) == 0) best[tid >> 6] = key;
     __syncthreads();
     if (tid == 0) {
@@ -183,11 +228,14 @@ void launch_rules(int kind, RuleArgs a, const aotk_logits_rule *rules, size_t ro
         for (size_t i = 0; i < n; i++) rr.rule[i] = rules[r0 + i];
         for (size_t i = n; i < (size_t)RULE_ROWS; i++) rr.rule[i] = aotk_logits_rule{};
         a.row0 = (uint32_t)r0;
+        a.tables = 0;
+        for (size_t i = 0; i < n; i++) a.tables |= (rr.rule[i].hist_len ? 1u : 0u) | (rr.rule[i].bias_len ? 2u : 0u);
+        const size_t lds = ((a.tables & 1) + (a.tables >> 1)) * RULE_SLICE * sizeof(uint32_t);
         const dim3 grid(slices, (unsigned)n);
         switch (kind) {
-        case AOTK_F32: k_rules<AOTK_F32><<<grid, RULE_THREADS, 0, s>>>(a, rr); break;
-        case AOTK_F16: k_rules<AOTK_F16><<<grid, RULE_THREADS, 0, s>>>(a, rr); break;
-        default: k_rules<AOTK_BF16><<<grid, RULE_THREADS, 0, s>>>(a, rr); break;
+        case AOTK_F32: k_rules<AOTK_F32><<<grid, RULE_THREADS, lds, s>>>(a, rr); break;
+        case AOTK_F16: k_rules<AOTK_F16><<<grid, RULE_THREADS, lds, s>>>(a, rr); break;
+        default: k_rules<AOTK_BF16><<<grid, RULE_THREADS, lds, s>>>(a, rr); break;
         }
     }
     if (tokens) k_rules_pick<<<(unsigned)rows, 64, 0, s>>>(a.keys, (int)slices, tokens);
