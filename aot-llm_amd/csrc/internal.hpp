@@ -258,7 +258,7 @@ size_t attention_scratch_bytes(size_t n_head, size_t head_dim, size_t ctx, size_
 // output. Writes out [n_head * head_dim].
 void launch_attention_decode(float *out, const QkvPost &p, size_t ctx_rows, size_t pos0, size_t window,
                              const int *pos_dev, float *scratch, hipStream_t s);
-// attend.hip: rows over a range that all sequences share, then a range of
+// attend.hip, attend.hpp: rows over a range that all sequences share, then a range of
 // their own (see there for what a row sees).
 struct AttendSeq {
     uint32_t row0, rows;  // rows of q and out, packed
@@ -298,18 +298,22 @@ struct AttendPlace {
     uint32_t block0, chunks;  // first block of the launch, runs of its key tiles
     uint64_t part0;           // first partial result, in rows
 };
+struct AttendView {
+    const void *ka, *va;  // range A: na prefix positions, or the sequence's own first ones
+    const void *k, *v;
+    uint64_t na, window, n_sink;
+    uint32_t run, causal;  // causal 0: every row sees all `len` positions
+    uint32_t block0, seq0;
+};
 struct AttendLaunch {
     const void *q;
     void *out;
-    const void *ka, *va, *k, *v;
     float *part_ml, *part_acc;
-    uint64_t na, window, n_sink;
-    uint32_t n_head, n_kv_head, n_seq, run;
+    uint32_t n_head, n_kv_head, n_seq, prefix_blocks;
     float scale_log2;
-    uint32_t causal;   // 0: every row sees all `len` positions
-    uint32_t sinks_a;  // range A is the sequence's own cache
-    uint32_t joined;   // every row has partial results elsewhere too
-    AttendPlace seq[ATTEND_SEQS];
+    uint32_t joined;      // every row has partial results of the prefix's blocks
+    AttendView range[2];  // the sequences' own ranges; the prefix
+    AttendPlace seq[ATTEND_SEQS + 1];  // the last: all rows, over the prefix
 };
 size_t attend_scratch_bytes(int kind, int head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n);
 void launch_attend(int kind, int head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n, void *scratch, hipStream_t s);
