@@ -31,6 +31,7 @@
 
 namespace aotk {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
@@ -215,6 +216,33 @@ struct AttSees {
     __device__ __forceinline__ bool operator()(int c) const { return (c <= hi) & ((c > lo) | (c < sink)); }
 };
 
+// Maximum and sum with the lane 16 or 32 away: swaps of 16-lane rows and of
+// halves in the registers, not through LDS.
+__device__ __forceinline__ f32x2 swap16(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f32x2{__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ f32x2 swap32(float x) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f32x2{__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ float max32(float x) {
+    const f32x2 r = swap32(x);
+    return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float max16(float x) {
+    const f32x2 r = swap16(x);
+    return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float sum32(float x) {
+    const f32x2 r = swap32(x);
+    return r[0] + r[1];
+}
+__device__ __forceinline__ float sum16(float x) {
+    const f32x2 r = swap16(x);
+    return r[0] + r[1];
+}
+
 // New running maximum of a row (in units of the exponent): the base to
 // subtract, and the factor for what was summed so far.
 __device__ __forceinline__ float att_base(float mc) { return mc == NEG_INF ? 0.0f : mc; }
@@ -385,9 +413,7 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
             }
 #pragma unroll
             for (int i = 0; i < NK / 4; i++) mx = fmaxf(mx, p[i]);
-            mx = fmaxf(mx, shfl_xor(mx, 16));
-            mx = fmaxf(mx, shfl_xor(mx, 32));
-            mx *= a.scale_log2;
+            mx = max32(max16(mx)) * a.scale_log2;
             if (__any(mx > mc[b] + RESCALE)) {
                 const float to = fmaxf(mx, mc[b]), f = att_shift(mc[b], to);
                 mc[b] = to;
@@ -465,8 +491,7 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
     float2 (*const l_ml)[ROWS] = (float2 (*)[ROWS])(lds + NW * ROWS * (D + 4) * sizeof(float));
 #pragma unroll
     for (int b = 0; b < RB; b++) {
-        sum[b] += shfl_xor(sum[b], 16);
-        sum[b] += shfl_xor(sum[b], 32);
+        sum[b] = sum32(sum16(sum[b]));
         if (g == 0) l_ml[wave][b * 16 + n] = make_float2(mc[b], sum[b]);
     }
     __syncthreads();
@@ -609,6 +634,35 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
         }
     };
 
+    // V's operands of step vi: f32, one key per half (accumulator register vi's)
+    // and four dimensions a lane and load; 16 bits, 16 keys. There lane l of a
+    // transposing read addresses key l % 16 / 4, dimensions 4 (l % 4).. of its 16
+    // lanes' 4 x 16 piece, and receives dimension l % 16 of the 4 keys.
+    constexpr int VN = F32 ? 16 : NK / 16, VG = F32 ? (S::NA + 3) / 4 : S::NA;
+    auto read_v = [&](int buf, int vi, u32x4 *f) {
+        if constexpr (F32) {
+            const float *row = (const float *)lv + (buf * NK + 8 * (vi / 4) + 4 * h + vi % 4) * S::VS + n * S::CW;
+#pragma unroll
+            for (int c = 0; c < VG; c++) {
+                if constexpr (S::CW == 2) {
+                    const u32x2 y = *(const u32x2 *)row;
+                    f[c] = u32x4{y[0], y[1], 0, 0};
+                } else {
+                    f[c] = *(const u32x4 *)(row + c * 128);
+                }
+            }
+        } else {
+            typedef __attribute__((address_space(3))) i16x4 *lds_i16x4;
+            const E *at = lv + (buf * NK + vi * 16 + 4 * h + (lane >> 2 & 3)) * S::VS + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+            for (int c = 0; c < VG; c++) {
+                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + c * 32)));
+                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + c * 32 + 8 * S::VS)));
+                f[c] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+            }
+        }
+    };
+
     if (tid < 6) l_bad[tid >> 1][tid & 1] = 0;
     AttTile<E> x = {}, nx = {};
     __syncthreads();
@@ -626,24 +680,41 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
             nx = att_tile<E, NK>(w, kv, t + 1);
             fetch(nx);
         }
+        // Operands come from LDS a group ahead of the products that take them:
+        // groups of four registers, two groups in flight, the order pinned.
         f32x16 sc[NK / 32];
+        constexpr int KG = S::QR / 4, KN = NK / 32 * KG;
+        u32x4 kf[2][4];
+        const E *const krow = lk + (buf * NK + n) * S::KS + (F32 ? 4 * h : 8 * h);
+        auto read_k = [&](int gi) {
 #pragma unroll
-        for (int kb = 0; kb < NK / 32; kb++) {
+            for (int e = 0; e < 4; e++) kf[gi & 1][e] = *(const u32x4 *)(krow + gi / KG * 32 * S::KS + (gi % KG * 4 + e) * (F32 ? 8 : 16));
+        };
+        read_k(0);
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[kb][i] = 0.0f;
-            const E *row = lk + (buf * NK + kb * 32 + n) * S::KS;
+        for (int gi = 0; gi < KN; gi++) {
+            const int kb = gi / KG;
+            if (gi + 1 < KN) read_k(gi + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (gi % KG == 0)
 #pragma unroll
-            for (int u = 0; u < S::QR; u++) {
-                const u32x4 kk = *(const u32x4 *)(row + (F32 ? 8 * u + 4 * h : 16 * u + 8 * h));
+                for (int i = 0; i < 16; i++) sc[kb][i] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u32x4 kk = kf[gi & 1][e], qq = q[gi % KG * 4 + e];
                 if constexpr (F32) {
 #pragma unroll
                     for (int c = 0; c < 4; c++)
-                        sc[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kk[c]), __uint_as_float(q[u][c]), sc[kb], 0, 0, 0);
+                        sc[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kk[c]), __uint_as_float(qq[c]), sc[kb], 0, 0, 0);
                 } else {
-                    sc[kb] = AttElem<KIND>::mma32(kk, q[u], sc[kb]);
+                    sc[kb] = AttElem<KIND>::mma32(kk, qq, sc[kb]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        // the first values, while the weights are formed
+        u32x4 vf[2][VG];
+        read_v(buf, 0, vf[0]);
         if (x.n < NK || x.ragged) {
             const AttSees sees(w, x, rel);
 #pragma unroll
@@ -656,7 +727,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
         for (int kb = 0; kb < NK / 32; kb++)
 #pragma unroll
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[kb][i]);
-        mx = fmaxf(mx, shfl_xor(mx, 32)) * a.scale_log2;
+        mx = max32(mx) * a.scale_log2;
         if (__any(mx > mc + RESCALE)) {
             const float to = fmaxf(mx, mc), f = att_shift(mc, to);
             mc = to;
@@ -674,37 +745,22 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                 sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale_log2, -base));
                 sum += sc[kb][i];
             }
-        if constexpr (F32) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float *row = (const float *)lv + (buf * NK + 8 * (i / 4) + 4 * h + i % 4) * S::VS + n * S::CW;
+        for (int vi = 0; vi < VN; vi++) {
+            if (vi + 1 < VN) read_v(buf, vi + 1, vf[(vi + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (F32) {
 #pragma unroll
-                for (int c = 0; c < S::NA; c += S::CW) {
-                    const float *at = row + c / S::CW * (32 * S::CW);
-                    float vv[S::CW];
-                    __builtin_memcpy(vv, __builtin_assume_aligned(at, S::CW * 4), S::CW * 4);
-#pragma unroll
-                    for (int e = 0; e < S::CW; e++) acc[c + e] = __builtin_amdgcn_mfma_f32_32x32x2f32(vv[e], sc[0][i], acc[c + e], 0, 0, 0);
-                }
-            }
-        } else {
-            typedef __attribute__((address_space(3))) i16x4 *lds_i16x4;
-#pragma unroll
-            for (int st = 0; st < NK / 16; st++) {
+                for (int c = 0; c < S::NA; c++)
+                    acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(vf[vi & 1][c / 4][c % 4]), sc[0][vi], acc[c], 0, 0, 0);
+            } else {
                 u32x4 p;
 #pragma unroll
-                for (int e = 0; e < 4; e++) p[e] = AttElem<KIND>::pair(sc[st / 2][st % 2 * 8 + 2 * e], sc[st / 2][st % 2 * 8 + 2 * e + 1]);
-                // lane l of a transposing read addresses key l % 16 / 4,
-                // dimensions 4 (l % 4).. of its 16 lanes' 4 x 16 piece, and
-                // receives dimension l % 16 of the 4 keys
-                const E *at = lv + (buf * NK + st * 16 + 4 * h + (lane >> 2 & 3)) * S::VS + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+                for (int e = 0; e < 4; e++) p[e] = AttElem<KIND>::pair(sc[vi / 2][vi % 2 * 8 + 2 * e], sc[vi / 2][vi % 2 * 8 + 2 * e + 1]);
 #pragma unroll
-                for (int c = 0; c < S::NA; c++) {
-                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + c * 32)));
-                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + c * 32 + 8 * S::VS)));
-                    acc[c] = AttElem<KIND>::mma32(u32x4{lo[0], lo[1], hi[0], hi[1]}, p, acc[c]);
-                }
+                for (int c = 0; c < S::NA; c++) acc[c] = AttElem<KIND>::mma32(vf[vi & 1][c], p, acc[c]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (x.ragged) {
             for (int half = 0; half < NK / 32; half++) {
@@ -743,7 +799,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
         slot = next;
         __syncthreads();
     }
-    sum += shfl_xor(sum, 32);
+    sum = sum32(sum);
     if ((uint32_t)(wave * 32 + n) >= w.nr) return;
     auto four = [&](auto f) {  // f(dimension, four accumulated values from it on)
 #pragma unroll
