@@ -59,7 +59,7 @@ static void att_cut(int kind, int head_dim, const AttendArgs &a, uint64_t na, bo
     // (f32, for every row) would cost more than the tiles of a run: c runs of
     // T tiles take T / c tile times and c times the traffic of one result.
     const bool narrow = p.shape <= 2;
-    const double want = narrow ? 1024 : 512, least = narrow ? 4 : 1;
+    const double want = 512, least = narrow ? 4 : 1;
     double cuts = want / (double)items;
     if (!narrow) {
         const double tile_us = 4.0 * p.rows_tile * p.nk * head_dim / (kind == AOTK_F32 ? 0.5e6 : 3.5e6);

@@ -536,14 +536,14 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
 // the next tile's loads in flight in registers while this one is multiplied.
 // LDS rows are padded so that the operand reads touch every bank once: K's
 // 16-byte reads of 32 rows by 16 bytes, 16-bit V's transposing reads (4 keys x
-// 16 dimensions per 16 lanes) by 32 bytes.
+// 32 dimensions per half wave) by 64 bytes.
 template <int KIND, int D>
 struct WideShape {
     static constexpr bool F32 = KIND == AOTK_F32;
     static constexpr int ESZ = F32 ? 4 : 2;
     static constexpr int NK = (F32 || D == 256) ? 32 : 64;
     static constexpr int KS = D + 16 / ESZ;              // LDS row of K, elements
-    static constexpr int VS = F32 ? D : D + 16;          // LDS row of V
+    static constexpr int VS = F32 ? D : D + 32;          // LDS row of V
     static constexpr int QR = F32 ? D / 8 : D / 16;      // 16-byte registers of q
     static constexpr int NA = D / 32;                    // accumulators of 32 dimensions x 32 rows
     static constexpr int CW = F32 ? (D == 64 ? 2 : 4) : 1;
@@ -680,28 +680,27 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
             nx = att_tile<E, NK>(w, kv, t + 1);
             fetch(nx);
         }
-        // Operands come from LDS a group ahead of the products that take them:
-        // groups of four registers, two groups in flight, the order pinned.
-        f32x16 sc[NK / 32];
-        constexpr int KG = S::QR / 4, KN = NK / 32 * KG;
-        u32x4 kf[2][4];
+        // The tile in pieces of 32 keys: the scores of a piece, the row's
+        // maximum, the weights, the values. Operands come from LDS a group
+        // ahead of the products that take them. With two pieces the second's
+        // scores are multiplied while the first's weights are formed, and the
+        // first's values while the second's are: matrix and vector
+        // instructions of one wave in turns.
+        constexpr int P = NK / 32, KG = S::QR / 4;
+        f32x16 sc[P];
+        u32x4 kf[2][4], vf[2][VG];
         const E *const krow = lk + (buf * NK + n) * S::KS + (F32 ? 4 * h : 8 * h);
-        auto read_k = [&](int gi) {
+        auto read_k = [&](int kb, int gi) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) kf[gi & 1][e] = *(const u32x4 *)(krow + gi / KG * 32 * S::KS + (gi % KG * 4 + e) * (F32 ? 8 : 16));
+            for (int e = 0; e < 4; e++) kf[(kb * KG + gi) & 1][e] = *(const u32x4 *)(krow + kb * 32 * S::KS + (gi * 4 + e) * (F32 ? 8 : 16));
         };
-        read_k(0);
-#pragma unroll
-        for (int gi = 0; gi < KN; gi++) {
-            const int kb = gi / KG;
-            if (gi + 1 < KN) read_k(gi + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            if (gi % KG == 0)
+        auto scores = [&](int kb, int gi) {
+            if (gi == 0)
 #pragma unroll
                 for (int i = 0; i < 16; i++) sc[kb][i] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const u32x4 kk = kf[gi & 1][e], qq = q[gi % KG * 4 + e];
+                const u32x4 kk = kf[(kb * KG + gi) & 1][e], qq = q[gi * 4 + e];
                 if constexpr (F32) {
 #pragma unroll
                     for (int c = 0; c < 4; c++)
@@ -710,45 +709,39 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                     sc[kb] = AttElem<KIND>::mma32(kk, qq, sc[kb]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // the first values, while the weights are formed
-        u32x4 vf[2][VG];
-        read_v(buf, 0, vf[0]);
-        if (x.n < NK || x.ragged) {
-            const AttSees sees(w, x, rel);
-#pragma unroll
-            for (int kb = 0; kb < NK / 32; kb++)
+        };
+        auto rescale = [&](int kb) {
+            if (x.n < NK || x.ragged) {
+                const AttSees sees(w, x, rel);
 #pragma unroll
                 for (int i = 0; i < 16; i++) sc[kb][i] = sees(kb * 32 + 8 * (i / 4) + 4 * h + i % 4) ? sc[kb][i] : NEG_INF;
-        }
-        float mx = NEG_INF;
-#pragma unroll
-        for (int kb = 0; kb < NK / 32; kb++)
+            }
+            float mx = NEG_INF;
 #pragma unroll
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[kb][i]);
-        mx = max32(mx) * a.scale_log2;
-        if (__any(mx > mc + RESCALE)) {
-            const float to = fmaxf(mx, mc), f = att_shift(mc, to);
-            mc = to;
-            sum *= f;
+            mx = max32(mx) * a.scale_log2;
+            if (__any(mx > mc + RESCALE)) {
+                const float to = fmaxf(mx, mc), f = att_shift(mc, to);
+                mc = to;
+                sum *= f;
 #pragma unroll
-            for (int c = 0; c < S::NA; c++)
+                for (int c = 0; c < S::NA; c++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) acc[c][i] *= f;
-        }
-        const float base = att_base(mc);
+                    for (int i = 0; i < 16; i++) acc[c][i] *= f;
+                if (kb == 1)  // the first piece's weights, not yet taken
 #pragma unroll
-        for (int kb = 0; kb < NK / 32; kb++)
+                    for (int i = 0; i < 16; i++) sc[0][i] *= f;
+            }
+        };
+        auto weights = [&](int kb) {
+            const float base = att_base(mc);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale_log2, -base));
                 sum += sc[kb][i];
             }
-#pragma unroll
-        for (int vi = 0; vi < VN; vi++) {
-            if (vi + 1 < VN) read_v(buf, vi + 1, vf[(vi + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto values = [&](int vi) {
             if constexpr (F32) {
 #pragma unroll
                 for (int c = 0; c < S::NA; c++)
@@ -760,7 +753,63 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
 #pragma unroll
                 for (int c = 0; c < S::NA; c++) acc[c] = AttElem<KIND>::mma32(vf[vi & 1][c], p, acc[c]);
             }
+        };
+        read_k(0, 0);
+#pragma unroll
+        for (int gi = 0; gi < KG; gi++) {
+            if (gi + 1 < KG) read_k(0, gi + 1);
+            else if (P > 1) read_k(1, 0);
             __builtin_amdgcn_sched_barrier(0);
+            scores(0, gi);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        rescale(0);
+        if constexpr (P == 1) {
+            read_v(buf, 0, vf[0]);
+            weights(0);
+#pragma unroll
+            for (int vi = 0; vi < VN; vi++) {
+                if (vi + 1 < VN) read_v(buf, vi + 1, vf[(vi + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                values(vi);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int gi = 0; gi < KG; gi++) {
+                if (gi + 1 < KG) read_k(1, gi + 1);
+                scores(1, gi);
+            }
+            weights(0);
+            asm volatile("" : "+v"(sc[0]), "+v"(sum));  // formed here, not where they are used
+#pragma unroll
+            for (int i = 0; i < KG * 4; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);             // a read from LDS
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a matrix product
+                __builtin_amdgcn_sched_group_barrier(0x002, 48 / (KG * 4), 0); // weights
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            read_v(buf, 0, vf[0]);
+            rescale(1);
+            __builtin_amdgcn_sched_barrier(0);
+            read_v(buf, 1, vf[1]);
+            values(0);
+            read_v(buf, 2, vf[0]);
+            values(1);
+            weights(1);
+            asm volatile("" : "+v"(sc[1]), "+v"(sum));
+#pragma unroll
+            for (int i = 0; i < 2 * S::NA; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 56 / (2 * S::NA), 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            read_v(buf, 3, vf[1]);
+            values(2);
+            __builtin_amdgcn_sched_barrier(0);
+            values(3);
         }
         if (x.ragged) {
             for (int half = 0; half < NK / 32; half++) {
