@@ -26,34 +26,46 @@ constexpr int RULE_PER = RULE_SLICE / RULE_THREADS;  // values per thread
 
 typedef uint32_t u32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// Rows start at any multiple of the element size: vector accesses that
-// promise no more alignment than that.
+// A thread's piece: 16 bytes of a row, at any multiple of the element size
+// (rows start anywhere), as four words.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+
 template <int KIND>
-struct RuleVec;
-template <>
-struct RuleVec<AOTK_F32> {
-    typedef float elem;
-    typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
-    static constexpr int N = 4;
-    static __device__ __forceinline__ float up(float x) { return x; }
-    static __device__ __forceinline__ float down(float x) { return x; }
-};
-template <>
-struct RuleVec<AOTK_F16> {
+struct RuleKind {
     typedef uint16_t elem;
-    typedef uint16_t vec __attribute__((ext_vector_type(8), aligned(2)));
-    static constexpr int N = 8;
-    static __device__ __forceinline__ float up(uint16_t x) { return f16_to_f32(x); }
+    static constexpr int N = 8;  // values of a piece
+    static constexpr uint32_t NONE = KIND == AOTK_F16 ? 0xFC00u : 0xFF80u;  // -inf
+    static __device__ __forceinline__ float up(uint32_t x) { return KIND == AOTK_F16 ? f16_to_f32(x) : bf16_to_f32(x & 0xFFFFu); }
     // one conversion, to nearest even (overflow to infinity)
-    static __device__ __forceinline__ uint16_t down(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+    static __device__ __forceinline__ uint32_t down(float x) {
+        if constexpr (KIND == AOTK_F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+        else return f32_to_bf16(x);
+    }
+    static __device__ __forceinline__ float get(const u32x4 &x, int i) { return up(i & 1 ? x[i / 2] >> 16 : x[i / 2]); }
+    static __device__ __forceinline__ void set(u32x4 &x, int i, float v) {
+        x[i / 2] = i & 1 ? (x[i / 2] & 0xFFFFu) | (down(v) << 16) : (x[i / 2] & 0xFFFF0000u) | down(v);
+    }
+    // values whose bit is 0 become -inf: bits to fields of ones, two a word
+    static __device__ __forceinline__ void allow(u32x4 &x, uint32_t bits) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t lo = (uint32_t)((int)(bits << (31 - 2 * i)) >> 31), hi = (uint32_t)((int)(bits << (30 - 2 * i)) >> 31);
+            const uint32_t m = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
+            x[i] = (x[i] & m) | ((NONE << 16 | NONE) & ~m);
+        }
+    }
 };
 template <>
-struct RuleVec<AOTK_BF16> {
-    typedef uint16_t elem;
-    typedef uint16_t vec __attribute__((ext_vector_type(8), aligned(2)));
-    static constexpr int N = 8;
-    static __device__ __forceinline__ float up(uint16_t x) { return bf16_to_f32(x); }
-    static __device__ __forceinline__ uint16_t down(float x) { return f32_to_bf16(x); }
+struct RuleKind<AOTK_F32> {
+    typedef float elem;
+    static constexpr int N = 4;
+    static __device__ __forceinline__ float get(const u32x4 &x, int i) { return __uint_as_float(x[i]); }
+    static __device__ __forceinline__ void set(u32x4 &x, int i, float v) { x[i] = __float_as_uint(v); }
+    static __device__ __forceinline__ void allow(u32x4 &x, uint32_t bits) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = (bits >> i) & 1u ? x[i] : 0xFF800000u;
+    }
 };
 
 // Pick key: the value's order in the high word, the complement of the token
@@ -104,16 +116,20 @@ __device__ __forceinline__ u32x4a4 rule_first(const uint32_t *list, uint32_t n) 
 }
 
 // Everything that a block reads is requested before the first wait: logits,
-// mask words, the heads of the lists. `tables`: what the launch's rows need,
-// 1 a count per token, 2 a bias per token (16 KB of LDS each).
+// mask words, the heads of the lists. The lists' tokens of the slice get a bit
+// each, so that a thread asks once for its whole piece whether any rule names a
+// value of it: nearly always none does, and the piece is masked and stored as
+// loaded. `tables`: what the launch's rows need, 1 a count per token, 2 a bias
+// per token (16 KB of LDS each).
 template <int KIND>
 __global__ __launch_bounds__(RULE_THREADS) void k_rules(RuleArgs a, RuleRows rr) {
-    typedef RuleVec<KIND> VT;
-    typedef typename VT::elem elem;
-    typedef typename VT::vec vec;
-    constexpr int N = VT::N, G = RULE_PER / N;
+    typedef RuleKind<KIND> K;
+    typedef typename K::elem elem;
+    constexpr int N = K::N, G = RULE_PER / N;
     extern __shared__ __align__(16) uint32_t tables[];
-    __shared__ uint64_t best[RULE_THREADS / 64];
+    __shared__ uint32_t named[RULE_SLICE / 32];
+    __shared__ float best[RULE_THREADS / 64];
+    __shared__ uint32_t first_at;
     const aotk_logits_rule r = rr.rule[blockIdx.y];
     const size_t row = (size_t)a.row0 + blockIdx.y;
     const uint32_t base = blockIdx.x * (uint32_t)RULE_SLICE;
@@ -125,86 +141,104 @@ __global__ __launch_bounds__(RULE_THREADS) void k_rules(RuleArgs a, RuleRows rr)
     const bool pen = r.hist_len > 0 && (r.repetition != 1.0f || r.presence != 0.0f || r.frequency != 0.0f);
     const bool biased = r.bias_len > 0;
 
-    vec x[G];
+    u32x4 x[G];
     uint32_t word[G];
     const uint32_t *mask = r.mask >= 0 ? a.mask + (size_t)r.mask * ((a.vocab + 31) / 32) + base / 32 : nullptr;
 #pragma unroll
     for (int g = 0; g < G; g++) {
         const uint32_t t = (g * RULE_THREADS + tid) * N;
-        if (t + N <= left) x[g] = *(const vec *)(src + t);
-        else
+        if (t + N <= left) {
+            x[g] = *(const u32x4a2 *)(src + t);
+        } else {  // the row ends inside the piece, or before it
+            x[g] = u32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < N; i++) x[g][i] = t + i < left ? src[t + i] : (elem)0;
-        word[g] = mask && t < left ? mask[t / 32] : ~0u;
+            for (int i = 0; i < N; i++)
+                if (t + i < left) {
+                    if constexpr (N == 4) x[g][i] = __float_as_uint(src[t + i]);
+                    else x[g][i / 2] |= (uint32_t)src[t + i] << (i % 2 * 16);
+                }
+        }
+        word[g] = mask && t < left ? mask[t / 32] >> (t % 32) : ~0u;
     }
     const u32x4a4 h0 = pen ? rule_first(a.hist + r.hist_off, r.hist_len) : u32x4a4{0, 0, 0, 0};
     const u32x4a4 b0 = biased ? rule_first(a.bias_id + r.bias_off, r.bias_len) : u32x4a4{0, 0, 0, 0};
 
+    if (tid == 0) first_at = ~0u;
     if (pen || biased) {
-        const u32x4a4 zero = {0, 0, 0, 0};
+        const u32x4 zero = {0, 0, 0, 0};
         for (int i = tid * 4; i < RULE_SLICE; i += RULE_THREADS * 4) {
-            if (pen) *(u32x4a4 *)(cnt + i) = zero;
-            if (biased) *(u32x4a4 *)(last + i) = zero;
+            if (pen) *(u32x4 *)(cnt + i) = zero;
+            if (biased) *(u32x4 *)(last + i) = zero;
         }
+        if (tid < RULE_SLICE / 32) named[tid] = 0;
         __syncthreads();
-        if (pen) rule_list(a.hist + r.hist_off, r.hist_len, base, h0, [&](uint32_t t, uint32_t) { atomicAdd(&cnt[t], 1u); });
-        if (biased) rule_list(a.bias_id + r.bias_off, r.bias_len, base, b0, [&](uint32_t t, uint32_t i) { atomicMax(&last[t], i + 1); });
+        if (pen)
+            rule_list(a.hist + r.hist_off, r.hist_len, base, h0, [&](uint32_t t, uint32_t) {
+                atomicAdd(&cnt[t], 1u);
+                atomicOr(&named[t / 32], 1u << (t % 32));
+            });
+        if (biased)
+            rule_list(a.bias_id + r.bias_off, r.bias_len, base, b0, [&](uint32_t t, uint32_t i) {
+                atomicMax(&last[t], i + 1);
+                atomicOr(&named[t / 32], 1u << (t % 32));
+            });
         __syncthreads();
     }
 
     float top = -__builtin_inff();
-    uint32_t at = 0;
 #pragma unroll
     for (int g = 0; g < G; g++) {
         const uint32_t t = (g * RULE_THREADS + tid) * N;
         if (t >= left) continue;
-        const uint32_t bits = word[g] >> (t % 32);
-        vec y = x[g];
         if (pen || biased) {
-            float v[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = VT::up(x[g][i]);
-            if (pen)
+            const uint32_t who = (named[t / 32] >> (t % 32)) & ((1u << N) - 1);
+            if (who)
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    const uint32_t c = cnt[t + i];
-                    if (c) v[i] = (v[i] > 0.0f ? v[i] / r.repetition : v[i] * r.repetition) - (r.presence + r.frequency * (float)c);
+                    if (!((who >> i) & 1u)) continue;
+                    float v = K::get(x[g], i);
+                    const uint32_t c = pen ? cnt[t + i] : 0, e = biased ? last[t + i] : 0;
+                    if (c) v = (v > 0.0f ? v / r.repetition : v * r.repetition) - (r.presence + r.frequency * (float)c);
+                    if (e) v = v + a.bias[(size_t)r.bias_off + e - 1];
+                    K::set(x[g], i, v);
                 }
-            if (biased)
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const uint32_t e = last[t + i];
-                    if (e) v[i] = v[i] + a.bias[(size_t)r.bias_off + e - 1];
-                }
-#pragma unroll
-            for (int i = 0; i < N; i++) y[i] = VT::down(v[i]);
         }
-        const elem none = VT::down(-__builtin_inff());
-#pragma unroll
-        for (int i = 0; i < N; i++) y[i] = (bits >> i) & 1u ? y[i] : none;
-        if (a.keys)
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const float v = VT::up(y[i]);
-                if (v > top && t + i < left) {
-                    top = v;
-                    at = t + i;
-                }
-            }
-        if (t + N <= left) *(vec *)(dst + t) = y;
-        else
+        uint32_t bits = word[g];
+        if (t + N > left) bits &= (1u << (left - t)) - 1;  // nothing behind the row's end is picked
+        if (mask || t + N > left) K::allow(x[g], bits);
+        if (t + N <= left) {
+            *(u32x4a2 *)(dst + t) = x[g];
+        } else {
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (t + i < left) dst[t + i] = y[i];
+                if (t + i < left) {
+                    if constexpr (N == 4) dst[t + i] = __uint_as_float(x[g][i]);
+                    else dst[t + i] = (uint16_t)(x[g][i / 2] >> (i % 2 * 16));
+                }
+        }
+        if (a.keys)  // NaN is passed over
+#pragma unroll
+            for (int i = 0; i < N; i++) top = fmaxf(top, K::get(x[g], i));
     }
     if (!a.keys) return;
-    uint64_t key = wave_max_key(top > -__builtin_inff() ? rule_key(top, base + at) : 0);
-    if ((tid & 63) == 0) best[tid >> 6] = key;
+    float most = top;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, shfl_xor(most, o));
+    if ((tid & 63) == 0) best[tid >> 6] = most;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < RULE_THREADS / 64; w++) key = best[w] > key ? best[w] : key;
-        a.keys[row * gridDim.x + blockIdx.x] = key;
+#pragma unroll
+    for (int w = 0; w < RULE_THREADS / 64; w++) most = fmaxf(most, best[w]);
+    if (top == most && most > -__builtin_inff()) {  // whoever holds it: the lowest token
+#pragma unroll
+        for (int g = G - 1; g >= 0; g--)
+#pragma unroll
+            for (int i = N - 1; i >= 0; i--) {
+                const uint32_t t = (g * RULE_THREADS + tid) * N + i;
+                if (t < left && K::get(x[g], i) == most) atomicMin(&first_at, t);
+            }
     }
+    __syncthreads();
+    if (tid == 0) a.keys[row * gridDim.x + blockIdx.x] = first_at == ~0u ? 0 : rule_key(most, base + first_at);
 }
 
 // One wave per row: the best of its slices' keys.
