@@ -319,23 +319,25 @@ size_t attend_scratch_bytes(int kind, int head_dim, const AttendArgs &a, const A
 void launch_attend(int kind, int head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n, void *scratch, hipStream_t s);
 
 // rules.hip
-constexpr int RULE_SLICE = 4096;  // tokens of one block
-constexpr int RULE_ROWS = 96;    // rows whose rules travel in one launch's arguments
-struct RuleRows {
-    aotk_logits_rule rule[RULE_ROWS];
+constexpr int RULE_SLICE = 4096;  // tokens that a block works on at once
+constexpr int RULE_FEW = 96;      // rows whose rules travel in the launch's arguments
+struct RulePick {  // all 0 between launches
+    uint64_t key;
+    uint32_t done, unused;
 };
 struct RuleArgs {
     void *out;
     const void *logits;
     size_t stride;  // elements between rows
-    uint32_t vocab, row0;
+    uint32_t vocab;
     uint32_t tables;  // set by launch_rules
     const uint32_t *hist, *bias_id, *mask;
     const float *bias;
-    uint64_t *keys;  // rules_scratch_bytes, null: no picks
+    uint32_t *tokens;  // null: no picks
+    RulePick *picks;   // one per row
+    const aotk_logits_rule *rules;  // more than RULE_FEW: where the GPU reads them
 };
-size_t rules_scratch_bytes(size_t rows, size_t vocab);
-void launch_rules(int kind, RuleArgs a, const aotk_logits_rule *rules, size_t rows, uint32_t *tokens, hipStream_t s);
+void launch_rules(int kind, RuleArgs a, const aotk_logits_rule *rules, size_t rows, hipStream_t s);
 
 void launch_add(float *x, const float *y, size_t n, hipStream_t s);
 void launch_rmsnorm_add(float *x, const float *y, const float *w, size_t n, size_t m, float eps, hipStream_t s);

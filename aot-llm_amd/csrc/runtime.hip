@@ -537,6 +537,50 @@ static int ops_workspace(size_t bytes) {
     return 0;
 }
 
+// Rules of the rows in pinned host memory, which the kernels read in place: a
+// few dozen bytes a block, for less than a copy ahead of the launch takes.
+static aotk_logits_rule *g_ops_rules = nullptr;
+static size_t g_ops_rules_n = 0;
+
+static int ops_rules(const aotk_logits_rule *rules, size_t n) {
+    if (n > g_ops_rules_n) {
+        if (g_ops_rules) (void)hipHostFree(g_ops_rules);
+        g_ops_rules = nullptr;
+        g_ops_rules_n = 0;
+        const size_t want = align_up(n, 128);
+        if (hipHostMalloc((void **)&g_ops_rules, want * sizeof(*rules), hipHostMallocDefault) != hipSuccess) {
+            (void)hipGetLastError();
+            g_ops_rules = nullptr;
+            return fail("hipHostMalloc for the rules of %zu rows failed", n);
+        }
+        g_ops_rules_n = want;
+    }
+    memcpy(g_ops_rules, rules, n * sizeof(*rules));
+    return 0;
+}
+
+// The picks' words of that many rows: 0 when they are made, and left at 0 by
+// every launch.
+static RulePick *g_ops_picks = nullptr;
+static size_t g_ops_picks_n = 0;
+
+static int ops_picks(size_t n) {
+    if (n <= g_ops_picks_n) return 0;
+    if (g_ops_picks) (void)hipFree(g_ops_picks);
+    g_ops_picks = nullptr;
+    g_ops_picks_n = 0;
+    const size_t want = align_up(n, 1024);
+    if (hipMalloc(&g_ops_picks, want * sizeof(RulePick)) != hipSuccess ||
+        hipMemsetAsync(g_ops_picks, 0, want * sizeof(RulePick), g_stream) != hipSuccess) {
+        (void)hipGetLastError();
+        if (g_ops_picks) (void)hipFree(g_ops_picks);
+        g_ops_picks = nullptr;
+        return fail("device memory for the picks of %zu rows failed", n);
+    }
+    g_ops_picks_n = want;
+    return 0;
+}
+
 static bool overlaps(const void *a, size_t an, const void *b, size_t bn) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return an && bn && x < y + bn && y < x + an;
@@ -706,6 +750,7 @@ int aotk_logits_rules(void *out_dev, const void *logits_dev, int kind, size_t ro
         const aotk_logits_rule &r = rules_host[i];
         if (!(r.repetition > 0.0f) || isinf(r.repetition)) return fail("%s: row %zu: a repetition penalty of %g", what, i, (double)r.repetition);
         if (!isfinite(r.presence) || !isfinite(r.frequency)) return fail("%s: row %zu: a penalty is not finite", what, i);
+        if (r.hist_len > 0x7fffffffu || r.bias_len > 0x7fffffffu) return fail("%s: row %zu: a list of more than 2^31 - 1 entries", what, i);
         if ((uint64_t)r.hist_off + r.hist_len > n_hist) return fail("%s: row %zu: history outside the %zu tokens", what, i, n_hist);
         if ((uint64_t)r.bias_off + r.bias_len > n_bias) return fail("%s: row %zu: biases outside the %zu entries", what, i, n_bias);
         if (r.mask < -1 || (r.mask >= 0 && (size_t)r.mask >= n_mask)) return fail("%s: row %zu: mask %d of %zu", what, i, r.mask, n_mask);
@@ -729,7 +774,7 @@ int aotk_logits_rules(void *out_dev, const void *logits_dev, int kind, size_t ro
     if (ensure_init()) return -1;
     DeviceScope dev;
     if (!dev.ok) return fail("%s: the device cannot be selected", what);
-    if (tokens_dev && ops_workspace(rules_scratch_bytes(rows, vocab))) return -1;
+    if ((tokens_dev && ops_picks(rows)) || (rows > (size_t)RULE_FEW && ops_rules(rules_host, rows))) return -1;
     RuleArgs a = {};
     a.out = out_dev;
     a.logits = logits_dev;
@@ -739,8 +784,10 @@ int aotk_logits_rules(void *out_dev, const void *logits_dev, int kind, size_t ro
     a.bias_id = bias_id_dev;
     a.bias = bias_dev;
     a.mask = mask_dev;
-    a.keys = tokens_dev ? (uint64_t *)g_ops_ws : nullptr;
-    launch_rules(kind, a, rules_host, rows, tokens_dev, g_stream);
+    a.rules = g_ops_rules;
+    a.tokens = tokens_dev;
+    a.picks = g_ops_picks;
+    launch_rules(kind, a, rules_host, rows, g_stream);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
     if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));

@@ -87,7 +87,8 @@ def call_rules(lib, change):
     (dict(stride=999), "stride"), (dict(rules=None), "null"), (dict(out=None), "null"), (dict(logits=None), "null"),
     (dict(repetition=0.0), "row 1"), (dict(repetition=-1.0), "row 1"), (dict(repetition=np.nan), "row 1"),
     (dict(repetition=np.inf), "row 1"), (dict(presence=np.nan), "not finite"), (dict(frequency=np.inf), "not finite"),
-    (dict(hist_off=8, hist_len=3), "history outside"), (dict(hist_off=2 ** 32 - 1, hist_len=2 ** 32 - 1), "history outside"),
+    (dict(hist_off=8, hist_len=3), "history outside"), (dict(hist_off=2 ** 32 - 1, hist_len=2 ** 31 - 1), "history outside"),
+    (dict(hist_len=2 ** 31, n_hist=2 ** 40), "more than"), (dict(bias_len=2 ** 32 - 1, n_bias=2 ** 40), "more than"),
     (dict(bias_off=1, bias_len=4), "biases outside"), (dict(mask=1), "null"), (dict(hist=None, hist_len=1), "null"),
     (dict(bias=None, bias_len=1), "null"), (dict(bias_id=None, bias_len=1), "null"), (dict(logits=OUT + 400), "overlaps"),
     (dict(tokens=OUT + 7996), "overlaps"), (dict(hist=OUT + 40), "overlaps"), (dict(tokens=KT), "overlaps"),
