@@ -913,12 +913,13 @@ __global__ __launch_bounds__(64 * att_waves(P), D == 256 || P == 3 ? 1 : 2) void
 // sequence's own range. A lane holds the weight of every 64th run; each wave
 // sums every WAVES-th run's accumulators, four loads in flight.
 template <int KIND, int D, int WAVES>
-__global__ __launch_bounds__(256) void k_join(AttendLaunch a, uint32_t prefix_chunks, uint32_t total, uint32_t row_begin) {
+__global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void k_join(AttendLaunch a, uint32_t prefix_chunks, uint32_t total, uint32_t row_begin) {
     constexpr int N = D / 64;
     typedef float vec __attribute__((ext_vector_type(N)));
-    __shared__ float l_acc[4][D];
+    constexpr int ROWS = WAVES > 4 ? 1 : 4 / WAVES;  // of a block
+    __shared__ float l_acc[ROWS * WAVES][D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % WAVES;
-    const uint32_t item = blockIdx.x * (4 / WAVES) + wave / WAVES;
+    const uint32_t item = blockIdx.x * ROWS + wave / WAVES;
     const uint32_t row = row_begin + item / a.n_head, head = item % a.n_head;
     const bool le = lane < (int)a.n_seq && a.seq[lane].row0 <= row;
     const uint32_t si = (uint32_t)__builtin_amdgcn_readfirstlane(__popcll(__ballot(le)) - 1);
@@ -1015,7 +1016,8 @@ template <int KIND>
 void att_join_kind(int head_dim, const AttendLaunch &a, uint32_t prefix_chunks, uint32_t total, uint32_t first_row, uint64_t items, uint32_t runs, hipStream_t s) {
     auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (runs >= 8) k_join<KIND, D, 4><<<(unsigned)items, 256, 0, s>>>(a, prefix_chunks, total, first_row);
+        if (runs >= 32) k_join<KIND, D, 16><<<(unsigned)items, 1024, 0, s>>>(a, prefix_chunks, total, first_row);
+        else if (runs >= 8) k_join<KIND, D, 4><<<(unsigned)items, 256, 0, s>>>(a, prefix_chunks, total, first_row);
         else k_join<KIND, D, 1><<<(unsigned)((items + 3) / 4), 256, 0, s>>>(a, prefix_chunks, total, first_row);
     };
     if (head_dim == 64) go(std::integral_constant<int, 64>());
