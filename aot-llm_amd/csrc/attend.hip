@@ -55,21 +55,31 @@ static void att_cut(int kind, int head_dim, const AttendArgs &a, uint64_t na, bo
     if (!items || !tiles) return;
     tiles *= a.n_kv_head;
     items *= a.n_kv_head;
-    // As many runs as fill the chip, unless writing and joining their results
-    // (f32, for every row) would cost more than the tiles of a run: c runs of
-    // T tiles take T / c tile times and c times the traffic of one result.
+    // As many runs as fill the chip (512 blocks are resident at two a CU), unless
+    // writing and joining their results (f32, for every row) would cost more than
+    // the tiles of a run: c runs of T tiles take T / c tile times and c times the
+    // traffic of one result. Measured around that optimum (times 0.7 / 1 / 1.5 of
+    // its c): 64 sequences behind 8192 bf16 56 / 52 / 57 us, 64 f32 rows in a 1024
+    // window 53 / 47 / 54 us. Few rows: runs of one tile a wave at least (of two: 27
+    // -> 30 us for a 1024 window, one f32 row).
     const bool narrow = p.shape <= 2;
     const double want = 512, least = narrow ? 4 : 1;
-    double cuts = want / (double)items;
-    if (!narrow) {
-        const double tile_us = 4.0 * p.rows_tile * p.nk * head_dim / (kind == AOTK_F32 ? 0.5e6 : 3.5e6);
-        const double part_us = (double)items * p.rows_tile * head_dim * 8 / 4e6;
-        const double most_cuts = sqrt((double)tiles / (double)items * tile_us / part_us);
-        cuts = cuts < most_cuts ? cuts : most_cuts;
+    const double each = (double)tiles / (double)items;  // of a row tile, on average
+    double run;
+    if ((double)items >= want) {
+        run = (double)tiles / want + 3;  // whole row tiles, but for those far longer than the others
+    } else {
+        double cuts = want / (double)items;
+        if (!narrow) {
+            const double tile_us = 4.0 * p.rows_tile * p.nk * head_dim / (kind == AOTK_F32 ? 0.5e6 : 3.5e6);
+            const double part_us = (double)items * p.rows_tile * head_dim * 8 / 4e6;
+            const double most_cuts = sqrt(each * tile_us / part_us);
+            cuts = cuts < most_cuts ? cuts : most_cuts;
+        }
+        run = ceil(each / floor(cuts < 1 ? 1 : cuts));
     }
-    if (cuts < 1) cuts = 1;
-    const double run = ceil((double)tiles / (double)items / floor(cuts));
-    p.run = items >= want ? 0x7fffffffu : (uint32_t)(run > least ? run : least);
+    run = run > least ? run : least;
+    p.run = run < 0x7fffffff ? (uint32_t)run : 0x7fffffffu;
 }
 
 static uint32_t att_chunks(const AttendArgs &a, uint64_t na, bool causal, const AttendSeq &s, uint32_t group, const AttPart &p) {

@@ -680,12 +680,10 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
             nx = att_tile<E, NK>(w, kv, t + 1);
             fetch(nx);
         }
-        // The tile in pieces of 32 keys: the scores of a piece, the row's
-        // maximum, the weights, the values. Operands come from LDS a group
-        // ahead of the products that take them. With two pieces the second's
-        // scores are multiplied while the first's weights are formed, and the
-        // first's values while the second's are: matrix and vector
-        // instructions of one wave in turns.
+        // Operands come from LDS a group ahead of the products that take them.
+        // (Pinning that order, and weaving the weights' vector instructions into
+        // the products of the other half of the tile, measured no faster: two
+        // waves a SIMD take turns by themselves.)
         constexpr int P = NK / 32, KG = S::QR / 4;
         f32x16 sc[P];
         u32x4 kf[2][4], vf[2][VG];
@@ -710,15 +708,19 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                 }
             }
         };
-        auto rescale = [&](int kb) {
+        auto rescale = [&]() {
             if (x.n < NK || x.ragged) {
                 const AttSees sees(w, x, rel);
 #pragma unroll
-                for (int i = 0; i < 16; i++) sc[kb][i] = sees(kb * 32 + 8 * (i / 4) + 4 * h + i % 4) ? sc[kb][i] : NEG_INF;
+                for (int kb = 0; kb < P; kb++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sc[kb][i] = sees(kb * 32 + 8 * (i / 4) + 4 * h + i % 4) ? sc[kb][i] : NEG_INF;
             }
             float mx = NEG_INF;
 #pragma unroll
-            for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[kb][i]);
+            for (int kb = 0; kb < P; kb++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[kb][i]);
             mx = max32(mx) * a.scale_log2;
             if (__any(mx > mc + RESCALE)) {
                 const float to = fmaxf(mx, mc), f = att_shift(mc, to);
@@ -728,18 +730,17 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                 for (int c = 0; c < S::NA; c++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[c][i] *= f;
-                if (kb == 1)  // the first piece's weights, not yet taken
-#pragma unroll
-                    for (int i = 0; i < 16; i++) sc[0][i] *= f;
             }
         };
-        auto weights = [&](int kb) {
+        auto weights = [&]() {
             const float base = att_base(mc);
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale_log2, -base));
-                sum += sc[kb][i];
-            }
+            for (int kb = 0; kb < P; kb++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale_log2, -base));
+                    sum += sc[kb][i];
+                }
         };
         auto values = [&](int vi) {
             if constexpr (F32) {
@@ -756,60 +757,17 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
         };
         read_k(0, 0);
 #pragma unroll
-        for (int gi = 0; gi < KG; gi++) {
-            if (gi + 1 < KG) read_k(0, gi + 1);
-            else if (P > 1) read_k(1, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            scores(0, gi);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int ki = 0; ki < P * KG; ki++) {
+            if (ki + 1 < P * KG) read_k((ki + 1) / KG, (ki + 1) % KG);
+            scores(ki / KG, ki % KG);
         }
-        rescale(0);
-        if constexpr (P == 1) {
-            read_v(buf, 0, vf[0]);
-            weights(0);
+        read_v(buf, 0, vf[0]);
+        rescale();
+        weights();
 #pragma unroll
-            for (int vi = 0; vi < VN; vi++) {
-                if (vi + 1 < VN) read_v(buf, vi + 1, vf[(vi + 1) & 1]);
-                __builtin_amdgcn_sched_barrier(0);
-                values(vi);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        } else {
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int gi = 0; gi < KG; gi++) {
-                if (gi + 1 < KG) read_k(1, gi + 1);
-                scores(1, gi);
-            }
-            weights(0);
-            asm volatile("" : "+v"(sc[0]), "+v"(sum));  // formed here, not where they are used
-#pragma unroll
-            for (int i = 0; i < KG * 4; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);             // a read from LDS
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a matrix product
-                __builtin_amdgcn_sched_group_barrier(0x002, 48 / (KG * 4), 0); // weights
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            read_v(buf, 0, vf[0]);
-            rescale(1);
-            __builtin_amdgcn_sched_barrier(0);
-            read_v(buf, 1, vf[1]);
-            values(0);
-            read_v(buf, 2, vf[0]);
-            values(1);
-            weights(1);
-            asm volatile("" : "+v"(sc[1]), "+v"(sum));
-#pragma unroll
-            for (int i = 0; i < 2 * S::NA; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 56 / (2 * S::NA), 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            read_v(buf, 3, vf[1]);
-            values(2);
-            __builtin_amdgcn_sched_barrier(0);
-            values(3);
+        for (int vi = 0; vi < VN; vi++) {
+            if (vi + 1 < VN) read_v(buf, vi + 1, vf[(vi + 1) & 1]);
+            values(vi);
         }
         if (x.ragged) {
             for (int half = 0; half < NK / 32; half++) {
