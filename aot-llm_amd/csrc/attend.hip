@@ -71,7 +71,9 @@ static void att_cut(int kind, int head_dim, const AttendArgs &a, uint64_t na, bo
     } else {
         double cuts = want / (double)items;
         if (!narrow) {
-            const double tile_us = 4.0 * p.rows_tile * p.nk * head_dim / (kind == AOTK_F32 ? 0.5e6 : 3.5e6);
+            // what a CU reaches; heads of 256 leave one wave a SIMD
+            const double rate = kind == AOTK_F32 ? 0.5e6 : (head_dim == 256 ? 2.0e6 : 3.5e6);
+            const double tile_us = 4.0 * p.rows_tile * p.nk * head_dim / rate;
             const double part_us = (double)items * p.rows_tile * head_dim * 8 / 4e6;
             const double most_cuts = sqrt(each * tile_us / part_us);
             cuts = cuts < most_cuts ? cuts : most_cuts;

@@ -505,19 +505,30 @@ int aotk_attention(float *out_dev, const float *q_dev, const float *k_cache_dev,
 // The operators for batches of continuations. They share one workspace, grown
 // on demand, and hold its lock until their work on the stream is done, so that
 // several threads may call them; a caller whose current device is another one
-// gets it back.
+// gets it back. A stream under capture is refused before anything is queued.
 static std::mutex g_ops_mutex;
 static void *g_ops_ws = nullptr;
 static size_t g_ops_ws_bytes = 0;
 
-struct DeviceScope {
+struct OpsScope {
+    std::lock_guard<std::mutex> hold;
     int before = -1;
     bool ok = false;
-    DeviceScope() {
+    explicit OpsScope(const char *what) : hold(g_ops_mutex) {
+        if (ensure_init()) return;
         if (hipGetDevice(&before) != hipSuccess) before = -1;
-        ok = before == g_device || hipSetDevice(g_device) == hipSuccess;
+        if (before != g_device && hipSetDevice(g_device) != hipSuccess) {
+            (void)fail("%s: device %d cannot be selected", what, g_device);
+            return;
+        }
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(g_stream, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) {
+            (void)fail("%s: the call waits for its result and cannot be captured", what);
+            return;
+        }
+        ok = true;
     }
-    ~DeviceScope() {
+    ~OpsScope() {
         if (before >= 0 && before != g_device) (void)hipSetDevice(before);
     }
 };
@@ -658,10 +669,8 @@ int aotk_attention_sinks(void *out_dev, const void *q_dev, const void *k_cache_d
     a.n_kv_head = (uint32_t)n_kv_head;
     a.scale = 1.0f / sqrtf((float)head_dim);
     const AttendSeq seq = {0, (uint32_t)m, pos0 + m, 0};
-    std::lock_guard<std::mutex> hold(g_ops_mutex);
-    if (ensure_init()) return -1;
-    DeviceScope dev;
-    if (!dev.ok) return fail("%s: the device cannot be selected", what);
+    OpsScope scope(what);
+    if (!scope.ok) return -1;
     return attend(what, kind, head_dim, a, &seq, 1);
 }
 
@@ -723,11 +732,8 @@ int aotk_attention_shared(void *out_dev, const void *q_dev, const void *k_prefix
     }
     int rc = -1;
     {
-        std::lock_guard<std::mutex> hold(g_ops_mutex);
-        if (!ensure_init()) {
-            DeviceScope dev;
-            rc = dev.ok ? attend(what, kind, head_dim, a, seqs, batch) : fail("%s: the device cannot be selected", what);
-        }
+        OpsScope scope(what);
+        if (scope.ok) rc = attend(what, kind, head_dim, a, seqs, batch);
     }
     free(seqs);
     return rc;
@@ -770,10 +776,8 @@ int aotk_logits_rules(void *out_dev, const void *logits_dev, int kind, size_t ro
     if ((out_dev != logits_dev && overlaps(out_dev, bytes, logits_dev, bytes)) ||
         (tokens_dev && (overlaps(tokens_dev, picks, logits_dev, bytes) || overlaps(tokens_dev, picks, out_dev, bytes))))
         return fail("%s: an output overlaps an input", what);
-    std::lock_guard<std::mutex> hold(g_ops_mutex);
-    if (ensure_init()) return -1;
-    DeviceScope dev;
-    if (!dev.ok) return fail("%s: the device cannot be selected", what);
+    OpsScope scope(what);
+    if (!scope.ok) return -1;
     if ((tokens_dev && ops_picks(rows)) || (rows > (size_t)RULE_FEW && ops_rules(rules_host, rows))) return -1;
     RuleArgs a = {};
     a.out = out_dev;

@@ -250,8 +250,11 @@ int aotk_attention(float *out_dev, const float *q_dev, const float *k_cache_dev,
  * AOTK_BF16, the same for all tensors of a call; scores, softmax statistics
  * and sums are f32, and results are rounded once to the kind, to nearest.
  * Pointers need the alignment of one element. Outputs must not overlap inputs
- * (aotk_logits_rules may write its logits in place). They may be called from
- * several host threads at once. */
+ * (aotk_logits_rules may write its logits in place). Like every call here they
+ * run on the library's stream and return when the result is there: what other
+ * streams write into their inputs has to be complete before the call, and a
+ * capture of the library's stream refuses them. They may be called from several
+ * host threads at once, and with another device current than the library's. */
 
 /* Attention of m rows at positions pos0..pos0+m-1 over a
  * [n_layer][ctx][kv_dim] cache, like aotk_attention, where the row at

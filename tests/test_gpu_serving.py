@@ -119,13 +119,14 @@ def test_sinks(aotk, kind, nh, nkv, hd):
 
 
 @KINDS
-@pytest.mark.parametrize("nh,nkv,hd", [(8, 4, 64), (8, 2, 128), (2, 2, 256)], ids=str)
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 4, 64), (8, 2, 128), (2, 2, 256), (2, 2, 128), (1, 1, 64)], ids=str)
 def test_sinks_values_not_finite_reach_only_rows_that_see_them(aotk, kind, nh, nkv, hd):
     """Positions that some rows of a call see and others do not hold NaN and
     infinities in K or V; also a long window's far rows."""
     for case, (pos0, m, window, n_sink, marks) in enumerate([
             (3, 40, 6, 2, {10: "vnan", 20: "vinf", 30: "knan"}), (100, 70, 16, 0, {101: "vinf", 150: "vnan", 169: "knan"}),
-            (0, 150, 0, 0, {70: "vnan", 149: "vinf"}), (64, 64, 32, 5, {64: "vnan", 4: "vinf", 127: "kinf"})]):
+            (0, 150, 0, 0, {70: "vnan", 149: "vinf"}), (40, 7, 5, 1, {41: "vinf", 44: "vnan", 46: "knan"}),
+            (40, 9, 0, 0, {30: "vinf", 42: "vnan", 47: "kinf"}), (64, 64, 32, 5, {64: "vnan", 4: "vinf", 127: "kinf"})]):
         rng = np.random.default_rng(77 + case)
         ctx = pos0 + m
         q = pack(rng.standard_normal((m, nh, hd)), kind)
@@ -273,6 +274,54 @@ def test_shared_many_sequences_and_rows_left_alone(aotk):
     got = out.to_numpy(np.float32).reshape(total + 3, nh, hd)
     assert (got[total:] == 7.0).all()
     check_rows(got[:total], q.astype(np.float64), shared_rows(kp, vp, kt, vt, 40, tail_len, rows, F32), F32)
+
+
+SHAPES = [  # nh, nkv, hd, prefix, tail lengths, rows: every pairing of the kernels' row tiles, prefix / tails
+    (2, 2, 64, 70, [9, 40, 3], None),  # 3 rows / 1
+    (8, 1, 128, 90, [30, 50, 7], None),  # 24 / 8
+    (20, 1, 128, 40, [5, 9], [1, 1]),  # 40 / 20 of 64
+    (4, 1, 64, 130, [40, 33, 2, 9], [9, 2, 1, 3]),  # 60 / 36
+    (8, 1, 256, 100, [33, 70, 5], None),  # 24 / 8, heads of 256
+    (24, 1, 256, 33, [64, 5], None),  # 48 / 24, heads of 256
+    (16, 2, 128, 300, [70, 1, 20] * 6, None),  # 144 / 8
+    (24, 1, 128, 200, [70, 33, 1, 9, 20, 64], None),  # 144 / 24
+    (4, 1, 128, 65, [50, 100, 3], [40, 90, 3]),  # 532 / 360
+    (6, 3, 256, 97, [50, 130, 3], [40, 90, 1]),  # 262 / 180, heads of 256
+    (128, 1, 64, 31, [2, 40], None),  # a group wider than a tile
+]
+
+
+@KINDS
+@pytest.mark.parametrize("nh,nkv,hd,n_prefix,tail_len,rows", SHAPES, ids=str)
+def test_shared_row_tiles(aotk, kind, nh, nkv, hd, n_prefix, tail_len, rows):
+    rng = np.random.default_rng(nh + hd)
+    nr = rows or [1] * len(tail_len)
+    tail_ctx = max(tail_len)
+    q, kp, vp, kt, vt = shared_inputs(rng, kind, nh, nkv, hd, n_prefix + 3, n_prefix, tail_ctx, tail_len, nr)
+    got = aotk.attention_shared(q, kp, vp, kt, vt, nh, nkv, hd, n_prefix + 3, n_prefix, tail_ctx, 1, tail_len, rows, kind)
+    check_rows(got, unpack(q, kind), shared_rows(kp, vp, kt, vt, n_prefix, tail_len, nr, kind), kind)
+
+
+@KINDS
+def test_shared_one_tail_far_longer_than_the_others(aotk, kind):
+    """A sequence whose run of keys is cut while the others' are whole, with
+    more blocks than fit the chip; one with many rows beside one with many keys."""
+    rng = np.random.default_rng(21)
+    nh, nkv, hd, n = 8, 2, 64, 300
+    tail_len = [3] * 150 + [1200] + [2] * 149
+    q, kp, vp = (pack(rng.standard_normal(s), kind) for s in ((n, nh, hd), (1, 5, nkv, hd), (1, 5, nkv, hd)))
+    kt, vt = (np.zeros((1, n, 1200, nkv, hd), q.dtype) for _ in range(2))
+    for c in (kt, vt):
+        for b, m in enumerate(tail_len):
+            c[0, b, :m] = pack(rng.standard_normal((m, nkv, hd)), kind)
+    got = aotk.attention_shared(q, kp, vp, kt, vt, nh, nkv, hd, 5, 5, 1200, 0, tail_len, None, kind)
+    keys = [np.concatenate([unpack(p[0], kind), unpack(t[0, b, :m], kind)]) for b, m in enumerate(tail_len) for p, t in ((kp, kt), (vp, vt))]
+    check_rows(got, unpack(q, kind), [(keys[2 * b], keys[2 * b + 1], np.ones(5 + m, bool)) for b, m in enumerate(tail_len)], kind)
+    kt, vt = (pack(rng.standard_normal((1, 3, 9000, nkv, hd)), kind) for _ in range(2))
+    lens, rows = [2, 9000, 1], [300, 1, 0]
+    q = pack(rng.standard_normal((301, nh, hd)), kind)
+    got = aotk.attention_shared(q, kp, vp, kt, vt, nh, nkv, hd, 5, 5, 9000, 0, lens, rows, kind)
+    check_rows(got, unpack(q, kind), shared_rows(kp, vp, kt, vt, 5, lens, rows, kind, 0), kind)
 
 
 def test_shared_without_rows_is_no_work(aotk):
@@ -519,3 +568,28 @@ def test_calls_from_several_threads(aotk):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_a_stream_under_capture_is_refused(aotk):
+    """Nothing is queued, and the capture goes on."""
+    import ctypes as C
+    hip = C.CDLL("libamdhip64.so")
+    stream, graph = C.c_void_p(aotk.stream()), C.c_void_p()
+    lib = aotk.abi.load()
+    b = aotk.DeviceBuffer.from_numpy(np.ones(4096, np.float32))
+    out = aotk.DeviceBuffer(4096)
+    table = aotk.logits_rules_table([{}])[0]
+    lens = np.array([1], np.uint32)
+    calls = [lambda: lib.aotk_attention_sinks(out.ptr, b.ptr, b.ptr, b.ptr, F32, 1, 1, 64, 4, 0, 3, 1, 0, 0),
+             lambda: lib.aotk_attention_shared(out.ptr, b.ptr, b.ptr, b.ptr, b.ptr, b.ptr, F32, 1, 1, 64, 4, 4, 4, 0, 1,
+                                               lens.ctypes.data, None),
+             lambda: lib.aotk_logits_rules(out.ptr, b.ptr, F32, 1, 64, 64, table.ctypes.data, None, 0, None, None, 0, None, 0, None)]
+    assert [c() for c in calls] == [0, 0, 0]
+    assert hip.hipStreamBeginCapture(stream, 1) == 0
+    try:
+        got = [(c(), lib.aotk_last_error()) for c in calls]
+    finally:
+        assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+        hip.hipGraphDestroy(graph)
+    assert all(rc == -1 and b"captured" in why for rc, why in got)
+    assert [c() for c in calls] == [0, 0, 0]
