@@ -48,6 +48,10 @@ constexpr float NEG_INF = -__builtin_inff();
 // then weights reach 2^8 instead of 1, which every type here holds, and the
 // accumulator is not rescaled.
 constexpr float RESCALE = 8.0f;
+// f16 weights are kept 2^6 times as large (2^14 at most): below 2^-14 an f16
+// loses bits, and a long row may have many weights that small beside one large.
+template <int KIND>
+constexpr float LIFT = KIND == AOTK_F16 ? 6.0f : 0.0f;
 
 template <int KIND>
 struct AttElem {
@@ -382,16 +386,16 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
                     if ((uint32_t)v_key(j) >= x.n) y = u32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
+                        bool ok;
                         if constexpr (F32) {
-                            if (!AttElem<KIND>::finite(y[e])) {
-                                y[e] = 0;
-                                bad |= 1u << v_key(j);
-                            }
+                            ok = AttElem<KIND>::finite(y[e]);
+                            y[e] = ok ? y[e] : 0;
                         } else {
                             const bool lo = AttElem<KIND>::finite(y[e]), hi = AttElem<KIND>::finite(y[e] >> 16);
                             y[e] &= (lo ? 0xFFFFu : 0u) | (hi ? 0xFFFF0000u : 0u);
-                            if (!lo || !hi) bad |= 1u << v_key(j);
+                            ok = lo & hi;
                         }
+                        bad |= (ok ? 0u : 1u) << v_key(j);
                     }
                 }
         }
@@ -421,7 +425,7 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
 #pragma unroll
                 for (int c = 0; c < S::NA; c++) acc[b][c] *= f;
             }
-            const float base = att_base(mc[b]);
+            const float base = att_base(mc[b]) - LIFT<KIND>;
 #pragma unroll
             for (int i = 0; i < NK / 4; i++) {
                 p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, -base));
@@ -474,7 +478,8 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
                             uint32_t bits;
                             if constexpr (F32) bits = __float_as_uint(y);
                             else bits = y;
-                            if (vis && !AttElem<KIND>::finite(bits)) acc[b][e][i] += pv * AttElem<KIND>::up(y);
+                            const float sum_with = acc[b][e][i] + pv * AttElem<KIND>::up(y);
+                            acc[b][e][i] = (vis & !AttElem<KIND>::finite(bits)) ? sum_with : acc[b][e][i];
                             __builtin_amdgcn_sched_barrier(0);  // one load at a time: registers for the paths that run
                         }
                 }
@@ -733,7 +738,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
             }
         };
         auto weights = [&]() {
-            const float base = att_base(mc);
+            const float base = att_base(mc) - LIFT<KIND>;
 #pragma unroll
             for (int kb = 0; kb < P; kb++)
 #pragma unroll
@@ -791,7 +796,8 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                             uint32_t bits;
                             if constexpr (F32) bits = __float_as_uint(y);
                             else bits = y;
-                            if (vis && !AttElem<KIND>::finite(bits)) acc[e][i] += pv * AttElem<KIND>::up(y);
+                            const float sum_with = acc[e][i] + pv * AttElem<KIND>::up(y);
+                            acc[e][i] = (vis & !AttElem<KIND>::finite(bits)) ? sum_with : acc[e][i];
                             __builtin_amdgcn_sched_barrier(0);
                         }
                 }

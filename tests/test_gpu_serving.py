@@ -172,6 +172,22 @@ def test_sinks_scores_far_apart(aotk, kind):
 
 
 @KINDS
+@pytest.mark.parametrize("m", [1, 40])
+def test_sinks_many_small_weights_beside_a_large_one(aotk, kind, m):
+    """65536 equal weights of 1.37 x 2^-18 of the largest, a quarter of the sum."""
+    hd, n = 64, 65536
+    c = np.sqrt(hd) / 8
+    q, k, v = np.zeros((m, 1, hd)), np.zeros((1, n, 1, hd)), np.ones((1, n, 1, hd))
+    q[:, :, :2] = 8, 1
+    k[0, 7, 0, :2] = 1.5 * c, np.log(2 ** 18 / 1.37) * 8 - 12
+    v[0, 7] = -1
+    qp, kp, vp = pack(q, kind), pack(k, kind), pack(v, kind)
+    got = aotk.attention_sinks(qp, kp, vp, 1, 1, hd, n, 0, n - m, m, 0, 0, kind)
+    k64, v64 = unpack(kp[0], kind), unpack(vp[0], kind)
+    check_rows(got, unpack(qp, kind), [(k64, v64, np.arange(n) <= n - m + i) for i in range(m)], kind)
+
+
+@KINDS
 def test_sinks_rows_whose_scores_are_all_minus_infinity(aotk, kind):
     """Like the formula: such a row is NaN (no weight to divide by)."""
     q = pack(np.ones((1, 2, 64)), kind)
