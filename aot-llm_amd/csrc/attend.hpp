@@ -13,10 +13,13 @@
 // maximum and sum are in-lane operations plus one or two exchanges), and the
 // accumulator layout of S^T is, up to the order of the keys, the operand layout
 // of P^T in O^T = V^T P^T. So the weights go from the first product to the
-// second in registers, and only V's operand is read in that order of keys. 16-bit
-// weights are rounded to the caches' type for the second product (half a step
-// each, against values that are themselves rounded to it); the sums take them
-// unrounded.
+// second in registers, and only V's operand is read in that order of keys.
+// 16-bit weights go into the second product in the caches' type. Up to 32 rows
+// as two parts, rounded and rest: bound by memory, the product of the rest is free
+// (one row, 32784 bf16 keys: 41.0 and 41.4 us, error 2.5e-3 and 1.6e-3). More rows
+// are bound by the products: there rounded, half a step each against values that
+// are themselves rounded so. The sum takes them rounded too, so that equal values
+// stay what they are (8192 rows: 460 and 475 us).
 //
 // A block takes one kv head, a tile of rows (all query heads of the group x
 // positions, heads fastest) and a run of key tiles. Where runs are cut or a
@@ -67,6 +70,24 @@ struct AttElem {
         } else {
             typedef __bf16 b2 __attribute__((ext_vector_type(2)));
             return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
+        }
+    }
+    // both values of a pair
+    static __device__ __forceinline__ float first(uint32_t x) {
+        if constexpr (KIND == AOTK_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)x);
+        else return __uint_as_float(x << 16);
+    }
+    static __device__ __forceinline__ float second(uint32_t x) {
+        if constexpr (KIND == AOTK_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(x >> 16));
+        else return __uint_as_float(x & 0xFFFF0000u);
+    }
+    static __device__ __forceinline__ float add_pair(uint32_t x, float sum) {  // sum + first + second, one instruction
+        if constexpr (KIND == AOTK_F16) {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), h2{(_Float16)1, (_Float16)1}, sum, false);
+        } else {
+            typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+            return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, x), __builtin_bit_cast(b2, 0x3F803F80u), sum, false);
         }
     }
     static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -374,33 +395,7 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
             }
         if (more) load_k(nx);
 
-        // values that no row may see, or only some rows, must not meet a
-        // weight of 0 as infinities or NaN
-        uint32_t bad = 0;
-        if (x.n < NK || x.ragged) {
-#pragma unroll
-            for (int j = 0; j < S::VK; j++)
-#pragma unroll
-                for (int h = 0; h < S::VL; h++) {
-                    u32x4 &y = v[j * S::VL + h];
-                    if ((uint32_t)v_key(j) >= x.n) y = u32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        bool ok;
-                        if constexpr (F32) {
-                            ok = AttElem<KIND>::finite(y[e]);
-                            y[e] = ok ? y[e] : 0;
-                        } else {
-                            const bool lo = AttElem<KIND>::finite(y[e]), hi = AttElem<KIND>::finite(y[e] >> 16);
-                            y[e] &= (lo ? 0xFFFFu : 0u) | (hi ? 0xFFFF0000u : 0u);
-                            ok = lo & hi;
-                        }
-                        bad |= (ok ? 0u : 1u) << v_key(j);
-                    }
-                }
-        }
-
-        u32x4 p16[RB];
+        u32x4 p16[RB], p16_rest[RB];
         float p32[RB][NK / 4];
 #pragma unroll
         for (int b = 0; b < RB; b++) {
@@ -432,9 +427,52 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
                 sum[b] += p[i];
             }
             if constexpr (!F32)
-                p16[b] = u32x4{AttElem<KIND>::pair(p[0], p[1]), AttElem<KIND>::pair(p[2], p[3]), AttElem<KIND>::pair(p[4], p[5]),
-                               AttElem<KIND>::pair(p[6], p[7])};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t y = AttElem<KIND>::pair(p[2 * i], p[2 * i + 1]);
+                    p16[b][i] = y;
+                    p16_rest[b][i] = AttElem<KIND>::pair(p[2 * i] - AttElem<KIND>::first(y), p[2 * i + 1] - AttElem<KIND>::second(y));
+                }
         }
+
+        // values that no row may see, or only some rows, must not meet a
+        // weight of 0 as infinities or NaN, nor any infinity the rest of a
+        // weight, whose sign is either
+        uint32_t bad = 0;
+        bool apart = x.n < NK || x.ragged;
+        if constexpr (!F32) {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 top = {0, 0};
+#pragma unroll
+            for (int i = 0; i < S::VK * S::VL; i++)
+#pragma unroll
+                for (int e = 0; e < (D == 64 ? 2 : 4); e++)
+                    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[i][e] & 0x7FFF7FFFu));
+            apart |= __any(!AttElem<KIND>::finite(top[0]) || !AttElem<KIND>::finite(top[1]));
+        }
+        if (apart) {
+#pragma unroll
+            for (int j = 0; j < S::VK; j++)
+#pragma unroll
+                for (int h = 0; h < S::VL; h++) {
+                    u32x4 &y = v[j * S::VL + h];
+                    if ((uint32_t)v_key(j) >= x.n) y = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        bool ok;
+                        if constexpr (F32) {
+                            ok = AttElem<KIND>::finite(y[e]);
+                            y[e] = ok ? y[e] : 0;
+                        } else {
+                            const bool lo = AttElem<KIND>::finite(y[e]), hi = AttElem<KIND>::finite(y[e] >> 16);
+                            y[e] &= (lo ? 0xFFFFu : 0u) | (hi ? 0xFFFF0000u : 0u);
+                            ok = lo & hi;
+                        }
+                        bad |= (ok ? 0u : 1u) << v_key(j);
+                    }
+                }
+        }
+
         if constexpr (F32) {
 #pragma unroll
             for (int c = 0; c < S::NA; c++)
@@ -452,11 +490,11 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
                 for (int j = 0; j < 4; j++)  // keys 2j and 2j + 1 of dimension c
                     vt[j] = __builtin_amdgcn_perm(v[(2 * j + 1) * S::VL + h][e], v[2 * j * S::VL + h][e], c % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int b = 0; b < RB; b++) acc[b][c] = AttElem<KIND>::mma16(vt, p16[b], acc[b][c]);
+                for (int b = 0; b < RB; b++) acc[b][c] = AttElem<KIND>::mma16(vt, p16_rest[b], AttElem<KIND>::mma16(vt, p16[b], acc[b][c]));
             }
         }
         // the keys whose values were taken out, for the rows that see them
-        if (x.n < NK || x.ragged) {
+        if (apart) {
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) bad |= __shfl_xor(bad, o, 64);
             bad = __builtin_amdgcn_readfirstlane(bad);
@@ -691,6 +729,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
         // waves a SIMD take turns by themselves.)
         constexpr int P = NK / 32, KG = S::QR / 4;
         f32x16 sc[P];
+        uint32_t p16[P * 8];  // 16 bits: the weights, two a word, in sc's order
         u32x4 kf[2][4], vf[2][VG];
         const E *const krow = lk + (buf * NK + n) * S::KS + (F32 ? 4 * h : 8 * h);
         auto read_k = [&](int kb, int gi) {
@@ -742,10 +781,19 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
 #pragma unroll
             for (int kb = 0; kb < P; kb++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale_log2, -base));
-                    sum += sc[kb][i];
+                for (int i = 0; i < 16; i++) sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale_log2, -base));
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // short chains of sums
+#pragma unroll
+            for (int i = 0; i < P * 8; i++) {
+                const float x = sc[i / 8][i % 8 * 2], y = sc[i / 8][i % 8 * 2 + 1];
+                if constexpr (F32) {
+                    part[i % 4] += x + y;
+                } else {
+                    p16[i] = AttElem<KIND>::pair(x, y);
+                    part[i % 4] = AttElem<KIND>::add_pair(p16[i], part[i % 4]);
                 }
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
         };
         auto values = [&](int vi) {
             if constexpr (F32) {
@@ -753,9 +801,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                 for (int c = 0; c < S::NA; c++)
                     acc[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(vf[vi & 1][c / 4][c % 4]), sc[0][vi], acc[c], 0, 0, 0);
             } else {
-                u32x4 p;
-#pragma unroll
-                for (int e = 0; e < 4; e++) p[e] = AttElem<KIND>::pair(sc[vi / 2][vi % 2 * 8 + 2 * e], sc[vi / 2][vi % 2 * 8 + 2 * e + 1]);
+                const u32x4 p = {p16[vi * 4], p16[vi * 4 + 1], p16[vi * 4 + 2], p16[vi * 4 + 3]};
 #pragma unroll
                 for (int c = 0; c < S::NA; c++) acc[c] = AttElem<KIND>::mma32(vf[vi & 1][c], p, acc[c]);
             }
@@ -781,11 +827,14 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                 while (bad) {
                     const int c = __builtin_ctz(bad) + 32 * half;
                     bad &= bad - 1;
-                    float pv = 0.0f;
+                    float pv = 0.0f;  // the key's weight
 #pragma unroll
-                    for (int kb = 0; kb < NK / 32; kb++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) pv = kb * 16 + i == (c / 32) * 16 + c % 32 / 8 * 4 + c % 4 ? sc[kb][i] : pv;
+                    for (int i = 0; i < P * 16; i++) {
+                        float y;
+                        if constexpr (F32) y = sc[0][i];
+                        else y = i % 2 ? AttElem<KIND>::second(p16[i / 2]) : AttElem<KIND>::first(p16[i / 2]);
+                        pv = i == (c / 32) * 16 + c % 32 / 8 * 4 + c % 4 ? y : pv;
+                    }
                     pv = __shfl(pv, n + 32 * (c / 4 % 2), 64);
                     const bool vis = sees(c);
 #pragma unroll

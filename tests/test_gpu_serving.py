@@ -151,6 +151,25 @@ def test_sinks_values_not_finite_reach_only_rows_that_see_them(aotk, kind, nh, n
 
 
 @KINDS
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (8, 2, 128), (2, 1, 256)], ids=str)
+@pytest.mark.parametrize("m", [1, 5, 200])
+def test_sinks_infinite_values_that_every_row_sees(aotk, kind, nh, nkv, hd, m):
+    """In tiles that lie wholly before the rows: infinities stay infinities,
+    two of both signs and a NaN become NaN, in their dimensions alone."""
+    rng = np.random.default_rng(11)
+    ctx = 300 + m
+    q = pack(rng.standard_normal((m, nh, hd)), kind)
+    k, v = rng.standard_normal((2, 1, ctx, nkv, hd))
+    for j, d, x in [(10, 5, np.inf), (99, 6, -np.inf), (20, 7, np.inf), (70, 7, -np.inf), (140, 9, np.nan)]:
+        v[0, j, :, d] = x
+    k, v = pack(k, kind), pack(v, kind)
+    got = aotk.attention_sinks(q, k, v, nh, nkv, hd, ctx, 0, 300, m, 0, 0, kind)
+    k64, v64 = unpack(k[0], kind), unpack(v[0], kind)
+    with np.errstate(invalid="ignore"):
+        check_rows(got, unpack(q, kind), [(k64, v64, np.arange(ctx) <= 300 + i) for i in range(m)], kind)
+
+
+@KINDS
 def test_sinks_scores_far_apart(aotk, kind):
     """One key far above the others, many equal keys far below the largest
     (weights of 2^-15 whose sum still counts), scores of hundreds."""
