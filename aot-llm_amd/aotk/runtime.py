@@ -340,8 +340,11 @@ def logits_rules_table(rules):
 
 def allowed_mask(tokens, vocab):
     """One row of aotk_logits_rules' masks that allows `tokens` only."""
+    ids = np.asarray(list(tokens), np.int64)
+    if ids.size and (ids.min() < 0 or ids.max() >= vocab):
+        raise ValueError(f"a token outside the vocabulary of {vocab}")
     bits = np.zeros((vocab + 31) // 32 * 32, np.uint8)
-    bits[np.asarray(list(tokens), np.int64)] = 1
+    bits[ids] = 1
     return np.packbits(bits, bitorder="little").view("<u4")
 
 

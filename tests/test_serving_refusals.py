@@ -124,6 +124,10 @@ def test_the_table_of_rules():
 def test_allowed_mask():
     m = runtime.allowed_mask([0, 31, 32, 69], 70)
     assert list(m) == [0x80000001, 1, 1 << 5]
+    assert list(runtime.allowed_mask([], 33)) == [0, 0]
+    for outside in (-1, 70, 95):
+        with pytest.raises(ValueError, match="outside"):
+            runtime.allowed_mask([3, outside], 70)
 
 
 def test_state_logits_of_no_state(lib):
