@@ -116,14 +116,23 @@ struct AttWhole {
 static AttWhole att_whole(int kind, int head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n) {
     AttWhole w = {};
     w.group = a.n_head / a.n_kv_head;
-    uint64_t total = 0, most = 0, with_rows = 0;
+    uint64_t total = 0, most = 0, with_rows = 0, own_tiles = 0;
     for (size_t i = 0; i < n; i++) {
         total += seqs[i].rows;
+        own_tiles += att_row_tiles(seqs[i].rows, w.group, 128);
         most = most > seqs[i].rows ? most : seqs[i].rows;
         with_rows += seqs[i].rows > 0;
     }
     w.total = (uint32_t)total;
-    w.grouped = a.n_prefix > 0 && with_rows > 1;
+    // Beyond 1024 tiles of 16-bit rows, each sequence's blocks read the prefix for
+    // themselves: the products bound them, and results of two parts for every row
+    // need not be joined (bf16, 32 heads over 4 of 64: 16 sequences of 512 rows behind
+    // 4096 323 -> 261 us, 16 of 1024 behind 512 277 -> 151). With fewer, and with f32
+    // (32 over 8 of 128: 8 of 1024 behind 4096 2403 -> 2863 us), sharing is faster.
+    // Sequences of few rows among them would waste tiles: a quarter at most.
+    const uint64_t packed = att_row_tiles((uint32_t)total, w.group, 128);
+    const bool alone = kind != AOTK_F32 && packed * a.n_kv_head >= 1024 && own_tiles * 4 <= packed * 5;
+    w.grouped = a.n_prefix > 0 && with_rows > 1 && !alone;
     w.own.shape = att_shape(most * w.group, head_dim);
     if (w.grouped) {
         w.prefix.shape = att_shape(total * w.group, head_dim);
@@ -212,10 +221,14 @@ void launch_attend(int kind, int head_dim, const AttendArgs &a, const AttendSeq 
          : kind == AOTK_F16 ? att_launch_kind<AOTK_F16>
                             : att_launch_kind<AOTK_BF16>)(head_dim, w.prefix.shape, w.own.shape, l, blocks, s);
         l.prefix_blocks = 0;  // done with the first sequences
-        if (parts)
+        // (a launch holds less than 2^32 threads)
+        const uint32_t most = (1u << 21) / a.n_head / 4 * 4;
+        for (uint32_t r = first_row; parts && r < last_row; r += most) {
+            const uint32_t rows = last_row - r < most ? last_row - r : most;
             (kind == AOTK_F32   ? att_join_kind<AOTK_F32>
              : kind == AOTK_F16 ? att_join_kind<AOTK_F16>
-                                : att_join_kind<AOTK_BF16>)(head_dim, l, w.prefix_chunks, w.total, first_row, (uint64_t)(last_row - first_row) * a.n_head, runs, s);
+                                : att_join_kind<AOTK_BF16>)(head_dim, l, w.prefix_chunks, w.total, r, (uint64_t)rows * a.n_head, runs, s);
+        }
     }
 }
 

@@ -359,6 +359,36 @@ def test_shared_one_tail_far_longer_than_the_others(aotk, kind):
     check_rows(got, unpack(q, kind), shared_rows(kp, vp, kt, vt, 5, lens, rows, kind, 0), kind)
 
 
+@KINDS
+@pytest.mark.parametrize("rows", [[1100, 1100, 1000, 1200], [4300, 1, 0, 99]], ids=str)
+def test_shared_many_rows_of_every_sequence(aotk, kind, rows):
+    """More than a thousand tiles of rows; a sample of the rows is checked."""
+    nh, nkv, hd, n_prefix, tail_len = 32, 4, 64, 70, [1200, 1100, 900, 1300]
+    rng = np.random.default_rng(33)
+    q, kp, vp, kt, vt = shared_inputs(rng, kind, nh, nkv, hd, 72, n_prefix, 1300, tail_len, rows)
+    got = aotk.attention_shared(q, kp, vp, kt, vt, nh, nkv, hd, 72, n_prefix, 1300, 1, tail_len, rows, kind)
+    ends = np.cumsum(rows)
+    some = sorted({int(x) for x in [0, *(ends - 1), *ends[:-1], *rng.integers(0, ends[-1], 30)]})
+    want = shared_rows(kp, vp, kt, vt, n_prefix, tail_len, rows, kind)
+    check_rows(got.reshape(q.shape)[some], unpack(q, kind)[some], [want[i] for i in some], kind)
+
+
+def test_shared_more_rows_than_one_join_takes(aotk):
+    """Two parts for each of 66000 x 32 rows."""
+    nh, nkv, hd, rows = 32, 4, 64, [33001, 32999]
+    rng = np.random.default_rng(34)
+    few = rng.standard_normal((250, nh, hd)).astype(np.float32)
+    q = np.tile(few, (264, 1, 1))
+    kp, vp = rng.standard_normal((2, 1, 3, nkv, hd)).astype(np.float32)
+    kt, vt = rng.standard_normal((2, 1, 2, 5, nkv, hd)).astype(np.float32)
+    got = aotk.attention_shared(q, kp, vp, kt, vt, nh, nkv, hd, 3, 3, 5, 0, [5, 2], rows, F32).reshape(q.shape)
+    some = [0, 249, 32995, 32998, 33000, 33001, 65533, 65534, 65535, 65536, 65537, 65998, 65999]
+    want = shared_rows(kp, vp, kt, vt, 3, [5, 2], rows, F32, 0)
+    check_rows(got[some], q[some].astype(np.float64), [want[i] for i in some], F32)
+    # rows that see the prefix alone: the same for the same query
+    assert (got[250:32500].reshape(-1, 250, nh, hd) == got[:250]).all()
+
+
 def test_shared_without_rows_is_no_work(aotk):
     z = np.zeros((1, 1, 1, 64), np.float32)
     got = aotk.attention_shared(np.zeros((0, 1, 64), np.float32), z, z, np.zeros((1, 2, 1, 1, 64), np.float32),
