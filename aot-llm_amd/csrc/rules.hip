@@ -11,7 +11,10 @@
 // to the logits' type at the end. Rows differ in every rule, so each row's
 // rules travel in the launch's arguments.
 //
-// A block takes one slice of RULE_SLICE tokens of one row. What names tokens
+// One read and one write of the logits bound it: 256 x 262144 bf16, 268 MB, 67 us
+// (4.0 TB/s; a large copy reaches 5.1), 64 x 128256 f32 18 us, 1 x 32000 5.7 us.
+//
+// A block takes slices of RULE_SLICE tokens of one row. What names tokens
 // in list order (history, biases) is turned into per-token tables in LDS:
 // every block scans the row's whole lists and keeps the entries of its slice,
 // counting with integer adds and taking the last bias by an integer maximum,
