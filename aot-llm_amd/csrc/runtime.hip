@@ -1329,11 +1329,10 @@ static const void *act_for(aotk_state *st, int kind, const float *f32) {
 }
 
 // The generated layer sequence (emit.rs:243-333 for m == 1, :167-237 for m > 1).
-static void run_layers(aotk_state *st, size_t m, size_t pos0, const int *pos_dev) {
+static void run_layers(aotk_state *st, size_t m, size_t pos0, const int *pos_dev, hipStream_t s) {
     aotk_model *M = st->m;
     const aotk_dims &d = M->spec.dims;
     const aotk_flags &f = M->spec.flags;
-    hipStream_t s = g_stream;
     size_t dim = d.dim, qd = d.n_head * d.head_dim, kv = d.n_kv_head * d.head_dim;
     bool normed = false;  // this layer's attention norm done by the previous layer's post-norm join
     for (size_t l = 0; l < d.n_layer; l++) {
@@ -1423,19 +1422,48 @@ static void run_layers(aotk_state *st, size_t m, size_t pos0, const int *pos_dev
     }
 }
 
-static void run_logits(aotk_state *st, size_t row) {
+static void run_logits(aotk_state *st, size_t row, hipStream_t s) {
     aotk_model *M = st->m;
     const aotk_dims &d = M->spec.dims;
-    launch_rmsnorm_quant(st->x + row * d.dim, M->output_norm, d.dim, 1, d.eps, outs_for(st, {M->output.kind}, st->xb), g_stream);
-    launch_matvec(M->output, act_for(st, M->output.kind, st->xb), 1, st->logits, nullptr, g_stream);
+    launch_rmsnorm_quant(st->x + row * d.dim, M->output_norm, d.dim, 1, d.eps, outs_for(st, {M->output.kind}, st->xb), s);
+    launch_matvec(M->output, act_for(st, M->output.kind, st->xb), 1, st->logits, nullptr, s);
 }
 
-static void run_decode_step(aotk_state *st, int want_logits) {
+static void run_decode_step(aotk_state *st, int want_logits, hipStream_t s) {
     aotk_model *M = st->m;
     const aotk_dims &d = M->spec.dims;
-    launch_embed(M->embd, st->ctl, 1, sqrtf((float)d.dim), M->spec.flags.embd_scale, st->x, g_stream);
-    run_layers(st, 1, 0, (const int *)(st->ctl + 1));
-    if (want_logits) run_logits(st, 0);
+    launch_embed(M->embd, st->ctl, 1, sqrtf((float)d.dim), M->spec.flags.embd_scale, st->x, s);
+    run_layers(st, 1, 0, (const int *)(st->ctl + 1), s);
+    if (want_logits) run_logits(st, 0, s);
+}
+
+// step(stream) as an executable graph. It is recorded on a stream of its own:
+// on the library's, which other threads' calls use meanwhile, their launches
+// would become part of the graph and their waits would break the capture.
+template <typename F>
+static int capture_step(hipGraphExec_t *exec, const char *what, F step) {
+    int before = g_device;  // (a thread starts with device 0)
+    HIPC(hipGetDevice(&before));
+    if (before != g_device) HIPC(hipSetDevice(g_device));
+    hipStream_t s = nullptr;
+    hipGraph_t graph = nullptr;
+    hipError_t e = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
+    if (e == hipSuccess) {
+        e = hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal);
+        if (e == hipSuccess) {
+            step(s);
+            e = hipStreamEndCapture(s, &graph);
+        }
+        if (e == hipSuccess) e = hipGraphInstantiate(exec, graph, nullptr, nullptr, 0);
+        if (graph) (void)hipGraphDestroy(graph);
+        (void)hipStreamDestroy(s);
+    }
+    if (before != g_device) (void)hipSetDevice(before);
+    if (e != hipSuccess) {
+        *exec = nullptr;
+        return fail("graph capture of the %s step failed: %s", what, hipGetErrorString(e));
+    }
+    return 0;
 }
 
 extern "C" {
@@ -1448,7 +1476,7 @@ int aotk_forward(aotk_state *st, uint32_t token, size_t pos, int want_logits) {
     st->ctl_host[0] = token;
     st->ctl_host[1] = (uint32_t)pos;
     HIPC(hipMemcpyAsync(st->ctl, st->ctl_host, 8, hipMemcpyHostToDevice, g_stream));
-    run_decode_step(st, want_logits);
+    run_decode_step(st, want_logits, g_stream);
     HIPC(hipGetLastError());
     HIPC(hipStreamSynchronize(g_stream));
     return 0;
@@ -1464,8 +1492,8 @@ int aotk_forward_batch(aotk_state *st, const uint32_t *tokens, size_t m, size_t 
     HIPC(hipMemcpyAsync(st->tokens, tokens, m * 4, hipMemcpyHostToDevice, g_stream));
     aotk_model *M = st->m;
     launch_embed(M->embd, st->tokens, m, sqrtf((float)d.dim), M->spec.flags.embd_scale, st->x, g_stream);
-    run_layers(st, m, pos0, nullptr);
-    if (want_logits) run_logits(st, m - 1);
+    run_layers(st, m, pos0, nullptr, g_stream);
+    if (want_logits) run_logits(st, m - 1, g_stream);
     HIPC(hipGetLastError());
     HIPC(hipStreamSynchronize(g_stream));
     return 0;
@@ -1505,27 +1533,16 @@ int aotk_generate_greedy(aotk_state *st, size_t pos, size_t n, uint32_t *tokens_
     st->ctl_host[3] = 0;
     HIPC(hipMemcpyAsync(st->ctl + 1, st->ctl_host + 1, 4, hipMemcpyHostToDevice, g_stream));
     HIPC(hipMemcpyAsync(st->ctl + 3, st->ctl_host + 3, 4, hipMemcpyHostToDevice, g_stream));
-    auto step = [&]() {
-        launch_argmax(st->logits, vocab, st->ctl + 2, st->am_ws, g_stream);
-        launch_advance(st->ctl, (int *)(st->ctl + 3), st->hist, st->ctl + 2, g_stream);
-        run_decode_step(st, 1);
-        launch_inc((int *)(st->ctl + 1), g_stream);
+    auto step = [&](hipStream_t s) {
+        launch_argmax(st->logits, vocab, st->ctl + 2, st->am_ws, s);
+        launch_advance(st->ctl, (int *)(st->ctl + 3), st->hist, st->ctl + 2, s);
+        run_decode_step(st, 1, s);
+        launch_inc((int *)(st->ctl + 1), s);
     };
-    if (n > 1 && !st->gen_exec && g_decode_graphs) {
-        hipGraph_t graph = nullptr;
-        HIPC(hipStreamBeginCapture(g_stream, hipStreamCaptureModeThreadLocal));
-        step();
-        hipError_t e = hipStreamEndCapture(g_stream, &graph);
-        if (e == hipSuccess) e = hipGraphInstantiate(&st->gen_exec, graph, nullptr, nullptr, 0);
-        if (graph) (void)hipGraphDestroy(graph);
-        if (e != hipSuccess) {
-            st->gen_exec = nullptr;
-            return fail("graph capture of the decode step failed: %s", hipGetErrorString(e));
-        }
-    }
+    if (n > 1 && !st->gen_exec && g_decode_graphs && capture_step(&st->gen_exec, "decode", step)) return -1;
     for (size_t g = 0; g + 1 < n; g++) {
         if (st->gen_exec) HIPC(hipGraphLaunch(st->gen_exec, g_stream));
-        else step();
+        else step(g_stream);
     }
     launch_argmax(st->logits, vocab, st->ctl + 2, st->am_ws, g_stream);
     launch_advance(st->ctl, (int *)(st->ctl + 3), st->hist, st->ctl + 2, g_stream);
@@ -1664,14 +1681,14 @@ int aotk_generate(aotk_state *st, aotk_sampler *sp, size_t pos, size_t n, const 
     st->ctl_host[3] = 0;
     HIPC(hipMemcpyAsync(st->ctl + 1, st->ctl_host + 1, 4, hipMemcpyHostToDevice, g_stream));
     HIPC(hipMemcpyAsync(st->ctl + 3, st->ctl_host + 3, 4, hipMemcpyHostToDevice, g_stream));
-    auto pick = [&]() {
-        launch_sample(p, g_stream);
-        launch_advance(st->ctl, (int *)(st->ctl + 3), st->hist, st->ctl + 2, g_stream);
+    auto pick = [&](hipStream_t s) {
+        launch_sample(p, s);
+        launch_advance(st->ctl, (int *)(st->ctl + 3), st->hist, st->ctl + 2, s);
     };
-    auto step = [&]() {
-        pick();
-        run_decode_step(st, 1);
-        launch_inc((int *)(st->ctl + 1), g_stream);
+    auto step = [&](hipStream_t s) {
+        pick(s);
+        run_decode_step(st, 1, s);
+        launch_inc((int *)(st->ctl + 1), s);
     };
     // the captured step bakes in the sampler's config and rng address
     const bool same = st->samp_exec && st->samp_rng == (const void *)sp->rng &&
@@ -1679,24 +1696,15 @@ int aotk_generate(aotk_state *st, aotk_sampler *sp, size_t pos, size_t n, const 
     if (n > 1 && !same && g_decode_graphs) {
         if (st->samp_exec) (void)hipGraphExecDestroy(st->samp_exec);
         st->samp_exec = nullptr;
-        hipGraph_t graph = nullptr;
-        HIPC(hipStreamBeginCapture(g_stream, hipStreamCaptureModeThreadLocal));
-        step();
-        hipError_t e = hipStreamEndCapture(g_stream, &graph);
-        if (e == hipSuccess) e = hipGraphInstantiate(&st->samp_exec, graph, nullptr, nullptr, 0);
-        if (graph) (void)hipGraphDestroy(graph);
-        if (e != hipSuccess) {
-            st->samp_exec = nullptr;
-            return fail("graph capture of the sampling step failed: %s", hipGetErrorString(e));
-        }
+        if (capture_step(&st->samp_exec, "sampling", step)) return -1;
         st->samp_cfg = sp->cfg;
         st->samp_rng = sp->rng;
     }
     for (size_t g = 0; g + 1 < n; g++) {
         if (st->samp_exec) HIPC(hipGraphLaunch(st->samp_exec, g_stream));
-        else step();
+        else step(g_stream);
     }
-    pick();
+    pick(g_stream);
     HIPC(hipGetLastError());
     HIPC(hipMemcpyAsync(tokens_out, st->hist, n * 4, hipMemcpyDeviceToHost, g_stream));
     HIPC(hipStreamSynchronize(g_stream));

@@ -254,7 +254,8 @@ int aotk_attention(float *out_dev, const float *q_dev, const float *k_cache_dev,
  * run on the library's stream and return when the result is there: what other
  * streams write into their inputs has to be complete before the call, and a
  * capture of the library's stream refuses them. They may be called from several
- * host threads at once, and with another device current than the library's. */
+ * host threads at once, also while a state generates in another, and with
+ * another device current than the library's. */
 
 /* Attention of m rows at positions pos0..pos0+m-1 over a
  * [n_layer][ctx][kv_dim] cache, like aotk_attention, where the row at

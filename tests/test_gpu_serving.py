@@ -658,3 +658,56 @@ def test_a_stream_under_capture_is_refused(aotk):
         hip.hipGraphDestroy(graph)
     assert all(rc == -1 and b"captured" in why for rc, why in got)
     assert [c() for c in calls] == [0, 0, 0]
+
+
+def test_calls_beside_a_state_that_generates(aotk):
+    """One thread generates on fresh states, each of which captures its decode
+    step (greedy) and its sampling step; another makes the three calls: what
+    both give is what they give alone."""
+    spec = aotk.configs.build("tiny-q4km")
+    model = aotk.Model(spec, seed=3)
+    prompt = aotk.configs.prompt_tokens(1, 6, spec.d["vocab"])
+    rng = np.random.default_rng(12)
+    q = rng.standard_normal((3, 8, 128)).astype(np.float32)
+    k, v = rng.standard_normal((2, 900, 2, 128)).astype(np.float32)
+    kt, vt = rng.standard_normal((2, 3, 8, 2, 128)).astype(np.float32)
+    x = rng.standard_normal((3, 9000)).astype(np.float32)
+    jobs = [lambda: aotk.attention_sinks(q, k, v, 8, 2, 128, 900, 0, 897, 3, 0, 0),
+            lambda: aotk.attention_shared(q, k, v, kt, vt, 8, 2, 128, 900, 900, 8, 0, [8, 1, 4]),
+            lambda: aotk.logits_rules(x, [{"history": [1, 2], "frequency": 1.0}] * 3)[0]]
+
+    def tokens():
+        st = aotk.State(model, 64, 8)
+        st.prompt(prompt, batch=8)
+        greedy = st.generate(len(prompt), 8)
+        st.prompt(prompt, batch=8)
+        return list(greedy) + list(st.generate_sampled(aotk.Sampler(temperature=1.0, top_k=8, seed=5), len(prompt), 8, prompt))
+
+    alone, alone_tokens = [j() for j in jobs], tokens()
+    wrong, errors, done = [], [], threading.Event()
+
+    def generate():
+        try:
+            for i in range(12):
+                if tokens() != alone_tokens:
+                    wrong.append(("tokens", i))
+        except Exception as e:  # noqa: BLE001
+            errors.append(repr(e))
+        done.set()
+
+    def operators():
+        try:
+            for i in range(3000):
+                if done.is_set():
+                    break
+                if not np.array_equal(jobs[i % 3](), alone[i % 3]):
+                    wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            errors.append(repr(e))
+
+    threads = [threading.Thread(target=f) for f in (generate, operators)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and not wrong, (errors, wrong)

@@ -1,0 +1,122 @@
+"""The host side of the operators for many continuations, on a HIP runtime
+that runs no kernels (host_hip.cpp): which stream they launch on while a state
+captures its decode step, which device is current afterwards, what is waited
+for when a launch fails. Each test is a process of its own."""
+import os
+import subprocess
+import sys
+import textwrap
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+PKG = os.path.join(os.path.dirname(HERE), "aot-llm_amd")
+
+COMMON = """
+import ctypes as C, sys, threading
+import numpy as np
+hip = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+for f in ("hh_launched", "hh_foreign", "hh_queued"):
+    getattr(hip, f).restype = C.c_long
+hip.hh_queued.argtypes = [C.c_void_p]
+sys.path.insert(0, sys.argv[2])
+import aotk
+lib = aotk.abi.load()
+
+mem = np.zeros(1 << 16, np.float32)  # the device's memory is the host's here
+P = mem.ctypes.data
+OUT = P + (1 << 17)
+lens = np.array([3, 2], np.uint32)
+table = aotk.logits_rules_table([{}, {}])[0]
+calls = {
+    "sinks": lambda: lib.aotk_attention_sinks(OUT, P, P + 4096, P + 8192, 0, 1, 1, 64, 4, 0, 3, 1, 0, 0),
+    "shared": lambda: lib.aotk_attention_shared(OUT, P, P + 4096, P + 8192, P + 16384, P + 32768, 0, 1, 1, 64, 4, 4, 4, 0, 2,
+                                                lens.ctypes.data, None),
+    "rules": lambda: lib.aotk_logits_rules(OUT, P, 0, 2, 64, 64, table.ctypes.data, None, 0, None, None, 0, None, 0, None),
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def stand_in(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("hip") / "libhost_hip.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-pthread", os.path.join(HERE, "host_hip.cpp"), "-o", so],
+                   check=True)
+    return so
+
+
+def run(stand_in, body, *args):
+    p = subprocess.run([sys.executable, "-c", COMMON + textwrap.dedent(body), stand_in, PKG, *args], capture_output=True, text=True,
+                       timeout=300)
+    assert p.returncode == 0, p.stdout + p.stderr
+
+
+@pytest.mark.parametrize("how", ["greedy", "sampled"])
+@pytest.mark.parametrize("order", ["capture first", "call first"])
+def test_a_state_that_captures_its_decode_step_beside_the_calls(stand_in, how, order):
+    """The state's capture takes no launch of another thread's call, and the
+    call is not refused for it; both orders of the two."""
+    run(stand_in, """
+        how, order = sys.argv[3:]
+        aotk.init(0)
+        model = aotk.Model(aotk.configs.build("tiny-q4km"), seed=3)
+        sampler = aotk.Sampler(temperature=1.0, top_k=4)
+        for name, call in calls.items():
+            failed, rc = [], []
+
+            def generate():
+                try:
+                    if how == "greedy":
+                        aotk.State(model, 32, 8).generate(0, 4)
+                    else:
+                        aotk.State(model, 32, 8).generate_sampled(sampler, 0, 4, [])
+                except aotk.AotkError as e:
+                    failed.append(str(e))
+
+            def operator():
+                rc.append((call(), lib.aotk_last_error()))
+
+            a, b = threading.Thread(target=generate), threading.Thread(target=operator)
+            hip.hh_arm(0)
+            if order == "capture first":
+                a.start()
+                assert hip.hh_reached(0, 10000)
+                b.start()
+                b.join(10)
+            else:
+                hip.hh_arm(1)
+                b.start()
+                assert hip.hh_reached(1, 10000)
+                a.start()
+                hip.hh_reached(0, 2000)  # unless the state waits for the call
+                hip.hh_open(1)
+                b.join(10)
+            hip.hh_open(0)
+            a.join(20)
+            b.join(20)
+            assert hip.hh_foreign() == 0, (name, "launches of the call are in the state's graph")
+            assert rc and rc[0][0] == 0, (name, rc)
+            assert not failed, (name, failed)
+    """, how, order)
+
+
+def test_a_capture_from_a_thread_with_another_device_current(stand_in):
+    """The step is captured on the library's device; the thread keeps its own."""
+    run(stand_in, """
+        hip.hh_devices(3)
+        aotk.init(2)
+        model = aotk.Model(aotk.configs.build("tiny-q4km"), seed=3)
+        now = []
+
+        def generate():
+            hip.hipSetDevice(1)
+            aotk.State(model, 32, 8).generate(0, 4)
+            d = C.c_int()
+            hip.hipGetDevice(C.byref(d))
+            now.append(d.value)
+
+        t = threading.Thread(target=generate)
+        t.start()
+        t.join()
+        assert hip.hh_captured_on() == 2 and now == [1], (hip.hh_captured_on(), now)
+    """)
