@@ -515,8 +515,9 @@ struct OpsScope {
     int before = -1;
     bool ok = false;
     explicit OpsScope(const char *what) : hold(g_ops_mutex) {
-        if (ensure_init()) return;
+        // (asked first: the library's initialisation selects its own)
         if (hipGetDevice(&before) != hipSuccess) before = -1;
+        if (ensure_init()) return;
         if (before != g_device && hipSetDevice(g_device) != hipSuccess) {
             (void)fail("%s: device %d cannot be selected", what, g_device);
             return;

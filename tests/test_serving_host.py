@@ -120,3 +120,17 @@ def test_a_capture_from_a_thread_with_another_device_current(stand_in):
         t.join()
         assert hip.hh_captured_on() == 2 and now == [1], (hip.hh_captured_on(), now)
     """)
+
+
+@pytest.mark.parametrize("name", ["sinks", "shared", "rules"])
+def test_the_callers_device_is_given_back_by_the_librarys_first_call(stand_in, name):
+    """That call initialises the library, on device 0."""
+    run(stand_in, """
+        hip.hh_devices(3)
+        hip.hipSetDevice(1)
+        now = C.c_int()
+        for turn in range(2):
+            assert calls[sys.argv[3]]() == 0, lib.aotk_last_error()
+            hip.hipGetDevice(C.byref(now))
+            assert now.value == 1, (turn, now.value)
+    """, name)
