@@ -527,6 +527,7 @@ struct OpsScope {
             (void)fail("%s: the call waits for its result and cannot be captured", what);
             return;
         }
+        (void)hipGetLastError();  // of earlier calls in this thread
         ok = true;
     }
     ~OpsScope() {

@@ -134,3 +134,12 @@ def test_the_callers_device_is_given_back_by_the_librarys_first_call(stand_in, n
             hip.hipGetDevice(C.byref(now))
             assert now.value == 1, (turn, now.value)
     """, name)
+
+
+@pytest.mark.parametrize("name", ["sinks", "shared", "rules"])
+def test_an_earlier_error_of_the_thread_is_not_the_calls(stand_in, name):
+    run(stand_in, """
+        assert calls[sys.argv[3]]() == 0
+        hip.hh_set_last_error(2)
+        assert calls[sys.argv[3]]() == 0, lib.aotk_last_error()
+    """, name)
