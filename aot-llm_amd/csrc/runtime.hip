@@ -530,6 +530,13 @@ struct OpsScope {
         (void)hipGetLastError();  // of earlier calls in this thread
         ok = true;
     }
+    // Waits for what was launched, also where a launch failed: the caller may
+    // free its buffers, and the next call takes the same workspace.
+    int finish(const char *what) {
+        const hipError_t launch = hipGetLastError(), wait = hipStreamSynchronize(g_stream);
+        const hipError_t e = launch != hipSuccess ? launch : wait;
+        return e == hipSuccess ? 0 : fail("%s: %s", what, hipGetErrorString(e));
+    }
     ~OpsScope() {
         if (before >= 0 && before != g_device) (void)hipSetDevice(before);
     }
@@ -631,12 +638,11 @@ static int check_heads(const char *what, size_t n_head, size_t n_kv_head, size_t
 static constexpr size_t ATTEND_MAX_ROWS = size_t(1) << 30;
 
 static int attend(const char *what, int kind, size_t head_dim, const AttendArgs &a, const AttendSeq *seqs, size_t n) {
+    OpsScope scope(what);
+    if (!scope.ok) return -1;
     if (ops_workspace(attend_scratch_bytes(kind, (int)head_dim, a, seqs, n))) return -1;
     launch_attend(kind, (int)head_dim, a, seqs, n, g_ops_ws, g_stream);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
-    if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
-    return 0;
+    return scope.finish(what);
 }
 
 extern "C" {
@@ -671,8 +677,6 @@ int aotk_attention_sinks(void *out_dev, const void *q_dev, const void *k_cache_d
     a.n_kv_head = (uint32_t)n_kv_head;
     a.scale = 1.0f / sqrtf((float)head_dim);
     const AttendSeq seq = {0, (uint32_t)m, pos0 + m, 0};
-    OpsScope scope(what);
-    if (!scope.ok) return -1;
     return attend(what, kind, head_dim, a, &seq, 1);
 }
 
@@ -732,11 +736,7 @@ int aotk_attention_shared(void *out_dev, const void *q_dev, const void *k_prefix
         seqs[b] = {row0, r, tail_len_host[b], b * tail_ctx};
         row0 += r;
     }
-    int rc = -1;
-    {
-        OpsScope scope(what);
-        if (scope.ok) rc = attend(what, kind, head_dim, a, seqs, batch);
-    }
+    const int rc = attend(what, kind, head_dim, a, seqs, batch);
     free(seqs);
     return rc;
 }
@@ -794,10 +794,7 @@ int aotk_logits_rules(void *out_dev, const void *logits_dev, int kind, size_t ro
     a.tokens = tokens_dev;
     a.picks = g_ops_picks;
     launch_rules(kind, a, rules_host, rows, g_stream);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
-    if (e != hipSuccess) return fail("%s: %s", what, hipGetErrorString(e));
-    return 0;
+    return scope.finish(what);
 }
 
 int aotk_argmax(const float *x_dev, size_t n, uint32_t *out_host) {

@@ -143,3 +143,33 @@ def test_an_earlier_error_of_the_thread_is_not_the_calls(stand_in, name):
         hip.hh_set_last_error(2)
         assert calls[sys.argv[3]]() == 0, lib.aotk_last_error()
     """, name)
+
+
+def test_a_launch_that_fails_is_reported_after_the_others_have_ended(stand_in):
+    """Of a call of several launches each one fails once: the call says so, and
+    nothing of it is left on the stream when it returns."""
+    run(stand_in, """
+        aotk.init(0)
+        stream = aotk.stream()
+        many = np.ones(130, np.uint32)
+        rules = aotk.logits_rules_table([{}] * 65540)[0]
+        big = np.zeros(65540 * 4, np.float32)
+        several = {
+            "sinks": lambda: lib.aotk_attention_sinks(OUT, P, P + 4096, P + 8192, 0, 1, 1, 64, 200, 0, 199, 1, 0, 0),
+            "shared": lambda: lib.aotk_attention_shared(OUT, P, P + 40960, P + 43008, P + 45056, P + 78848, 0, 1, 1, 64, 4, 4, 1, 0,
+                                                        130, many.ctypes.data, None),
+            "rules": lambda: lib.aotk_logits_rules(big.ctypes.data, big.ctypes.data, 0, 65540, 4, 4, rules.ctypes.data, None, 0, None,
+                                                   None, 0, None, 0, None),
+        }
+        for name, call in several.items():
+            before = hip.hh_launched()
+            assert call() == 0, (name, lib.aotk_last_error())
+            n = hip.hh_launched() - before
+            assert n > 1, (name, n)
+            for i in range(n):
+                hip.hh_fail_launch(i + 1)
+                assert call() == -1, (name, i)
+                assert b"an error of the stand-in" in lib.aotk_last_error()
+                assert hip.hh_queued(stream) == 0, (name, i, "launches that nothing has waited for")
+            assert call() == 0, (name, lib.aotk_last_error())
+    """)
