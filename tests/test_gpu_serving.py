@@ -711,3 +711,57 @@ def test_calls_beside_a_state_that_generates(aotk):
     for t in threads:
         t.join()
     assert not errors and not wrong, (errors, wrong)
+
+
+# --------------------------------------------- many slices, rows and launches
+def rules_of_rows(rng, rows, vocab, n_mask):
+    rules = []
+    for i in range(rows):
+        h = [int(t) for t in rng.integers(0, vocab, int(rng.integers(0, 50)))]
+        b = [(int(t), float(np.float32(s))) for t, s in zip(rng.integers(0, vocab, 9), rng.standard_normal(9) * 5)]
+        rules.append({"repetition": [1.0, 1.3, 0.7][i % 3], "presence": [0.0, 0.5][i % 2], "frequency": [0.25, 0.0, -0.1][i % 3],
+                      "history": h if i % 4 != 3 else [], "bias": b if i % 5 != 1 else [], "mask": i % (n_mask + 1) - 1})
+    return rules
+
+
+@KINDS
+@pytest.mark.parametrize("rows,vocab", [(70, 70001), (70, 69001), (1100, 9000)], ids=str)
+def test_rules_blocks_of_several_slices(aotk, kind, rows, vocab):
+    """More rows x slices than blocks: 9 blocks of 2 slices a row, the last of
+    them short or alone, and one block a row. The largest values lie in any
+    slice, some twice, next to each other or slices apart."""
+    rng = np.random.default_rng(rows + vocab)
+    x = rng.standard_normal((rows, vocab)) * 3
+    for i in range(rows):
+        at = [int(t) for t in rng.integers(0, vocab, 1 + i % 3)] + [vocab - 1] * (i % 4 == 0)
+        x[i, at + ([min(at[0] + 1, vocab - 1)] if i % 5 == 0 else [])] = 100.0
+    masks = rng.integers(0, 1 << 32, (2, (vocab + 31) // 32), dtype=np.uint32)
+    check_rules(aotk, pack(x, kind), rules_of_rows(rng, rows, vocab, 2), masks, kind)
+
+
+@KINDS
+def test_rules_of_more_rows_than_the_arguments_hold(aotk, kind):
+    """Calls of growing and shrinking batches, each with rules of its own."""
+    rng = np.random.default_rng(40)
+    for rows, vocab in ((97, 1500), (300, 700), (97, 4100), (96, 900), (1200, 300), (130, 5000)):
+        x = pack(rng.standard_normal((rows, vocab)) * 3, kind)
+        masks = rng.integers(0, 1 << 32, (3, (vocab + 31) // 32), dtype=np.uint32)
+        check_rules(aotk, x, rules_of_rows(rng, rows, vocab, 3), masks, kind)
+
+
+def test_rules_of_more_rows_than_a_launch(aotk):
+    """65535 rows in the first launch: values and picks of all, exactly."""
+    rows, vocab = 65540, 40
+    rng = np.random.default_rng(41)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    masks = rng.integers(0, 1 << 32, (2, 2), dtype=np.uint32)
+    masks[0] = 0
+    i = np.arange(rows)
+    got, tok = aotk.logits_rules(x, [{"presence": 0.25 * (n % 7), "history": [n % vocab], "mask": n % 3 - 1} for n in range(rows)], masks)
+    want = x.copy()
+    want[i, i % vocab] -= (0.25 * (i % 7)).astype(np.float32)
+    bits = np.unpackbits(masks.view(np.uint8), axis=1, bitorder="little")[:, :vocab]
+    for m in range(2):
+        want[i % 3 == m + 1] = np.where(bits[m], want[i % 3 == m + 1], -np.inf)
+    assert np.array_equal(got, want)
+    assert np.array_equal(tok, np.where(want.max(1) > -np.inf, want.argmax(1), 0xFFFFFFFF))
