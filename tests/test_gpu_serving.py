@@ -765,3 +765,39 @@ def test_rules_of_more_rows_than_a_launch(aotk):
         want[i % 3 == m + 1] = np.where(bits[m], want[i % 3 == m + 1], -np.inf)
     assert np.array_equal(got, want)
     assert np.array_equal(tok, np.where(want.max(1) > -np.inf, want.argmax(1), 0xFFFFFFFF))
+
+
+# ------------------------------------------------------- weights and range
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("what,nh,hd", [("sinks", 1, 64), ("sinks", 16, 128), ("sinks", 16, 256), ("sinks", 32, 128),
+                                        ("sinks", 32, 64), ("shared", 8, 256), ("shared", 8, 128), ("shared", 16, 64)], ids=str)
+def test_weights_of_few_rows_keep_both_parts(aotk, kind, what, nh, hd):
+    """Up to 32 rows (16 with heads of 256) a 16-bit weight enters the second
+    product as its rounding and the rest's rounding: off by e^2, not by e. Two
+    sets of keys, values 1 and -1, whose weights differ by less than half a step
+    of the type: rounded weights alone would give 0."""
+    e = HALF_STEP[kind]
+    delta = {BF16: 0.0015, F16: 2e-4}[kind]  # e^-delta is nearer to 1 than to the type's next value below
+    n = 64
+    batch = 1 if what == "sinks" else 2
+    q = np.zeros((batch, nh, hd))
+    q[..., 0] = 1
+    k, v = np.zeros((n, 1, hd)), np.ones((n, 1, hd))
+    k[::2, 0, 0] = delta * np.sqrt(hd)
+    v[1::2] = -1
+    q, k, v = pack(q, kind), pack(k, kind), pack(v, kind)
+    if what == "sinks":
+        got = aotk.attention_sinks(q, k, v, nh, 1, hd, n, 0, n - 1, 1, 0, 0, kind)
+    else:
+        tails = [np.stack([x[44:], x[44:]]) for x in (k, v)]
+        got = aotk.attention_shared(q, k[:44], v[:44], *tails, nh, 1, hd, 44, 44, 20, 0, [20, 20], None, kind)
+    q64, k64, v64 = (unpack(x, kind) for x in (q, k, v))
+    s = k64[:, 0, 0] / np.sqrt(hd)
+    w = np.exp(s - s.max())
+    rounded = np.abs((unpack(pack(w, kind), kind) @ v64[:, 0, 0]) / w.sum() - (w @ v64[:, 0, 0]) / w.sum())
+    for b in range(batch):
+        want, tol = attend64(q64[b], k64, v64, np.ones(n, bool))
+        # the rest's rounding, e of at most e of a weight, and f16's smallest steps
+        tol = tol + 1.01 * e * e + (n * 2.0 ** -31 if kind == F16 else 0)
+        assert (rounded > 4 * (tol + np.abs(want) * e)).all()
+        near(unpack(got, kind).reshape(q.shape)[b], want, tol, 0.0, kind)
