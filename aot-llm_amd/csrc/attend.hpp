@@ -48,13 +48,21 @@ typedef uint32_t u32x2e __attribute__((ext_vector_type(2), aligned(2)));
 
 constexpr float NEG_INF = -__builtin_inff();
 // The running maximum moves only when a row's grows by more than 2^8: until
-// then weights reach 2^8 instead of 1, which every type here holds, and the
-// accumulator is not rescaled.
+// then weights are up to 2^8 times too large, and the accumulator is not rescaled.
 constexpr float RESCALE = 8.0f;
-// f16 weights are kept 2^6 times as large (2^14 at most): below 2^-14 an f16
-// loses bits, and a long row may have many weights that small beside one large.
+// Weights are kept 2^LIFT times as large. f16: 2^6 (2^14 at most), since below
+// 2^-14 an f16 loses bits, and a long row may have many weights that small beside
+// one large; its values are too small to overflow. The other types hold values as
+// large as f32 itself: at 2^-8 their weights are at most 1, and the sums overflow
+// where those of the formula do. bf16 takes the 2^-8 in the exponent; there it
+// would cost f32 weights two bits, which are multiplied by it instead.
 template <int KIND>
-constexpr float LIFT = KIND == AOTK_F16 ? 6.0f : 0.0f;
+constexpr float LIFT = KIND == AOTK_F16 ? 6.0f : (KIND == AOTK_BF16 ? -RESCALE : 0.0f);
+template <int KIND>
+__device__ __forceinline__ float att_weight(float score, float scale_log2, float base) {
+    const float w = __builtin_amdgcn_exp2f(fmaf(score, scale_log2, -base));
+    return KIND == AOTK_F32 ? w * 0x1p-8f : w;
+}
 
 template <int KIND>
 struct AttElem {
@@ -426,7 +434,7 @@ __device__ __forceinline__ void attend_narrow(const AttendLaunch &a, bool prefix
             const float base = att_base(mc[b]) - LIFT<KIND>;
 #pragma unroll
             for (int i = 0; i < NK / 4; i++) {
-                p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], a.scale_log2, -base));
+                p[i] = att_weight<KIND>(p[i], a.scale_log2, base);
                 sum[b] += p[i];
             }
             if constexpr (!F32)
@@ -788,7 +796,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
 #pragma unroll
             for (int kb = 0; kb < P; kb++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale_log2, -base));
+                for (int i = 0; i < 16; i++) sc[kb][i] = att_weight<KIND>(sc[kb][i], a.scale_log2, base);
             float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // short chains of sums
 #pragma unroll
             for (int i = 0; i < P * 8; i++) {

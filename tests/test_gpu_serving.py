@@ -801,3 +801,27 @@ def test_weights_of_few_rows_keep_both_parts(aotk, kind, what, nh, hd):
         tol = tol + 1.01 * e * e + (n * 2.0 ** -31 if kind == F16 else 0)
         assert (rounded > 4 * (tol + np.abs(want) * e)).all()
         near(unpack(got, kind).reshape(q.shape)[b], want, tol, 0.0, kind)
+
+
+@pytest.mark.parametrize("kind", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("m", [1, 40, 70])
+def test_large_values_overflow_no_earlier_than_the_formula(aotk, kind, hd, m):
+    """512 values of up to 4e35: their sum with weights of at most 1 stays in
+    f32's range. The latest keys score 5.2 above the earliest, so that a
+    maximum that lags behind would give them weights of 180."""
+    nh, n = 512, 512  # so many heads that a block takes all keys of its own
+    rng = np.random.default_rng(17)
+    q = np.zeros((m, nh, hd))
+    q[..., 0] = np.sqrt(hd)
+    k, v = np.zeros((n, nh, hd), np.float32), rng.uniform(2e35, 4e35, (n, nh, hd)).astype(np.float32)
+    k[128:, :, 0] = 5.2
+    q, k, v = pack(q, kind), pack(k, kind), pack(v, kind)
+    got = unpack(aotk.attention_sinks(q, k, v, nh, nh, hd, n, 0, n - m, m, 0, 0, kind), kind).reshape(m, nh, hd)
+    assert (~np.isfinite(got)).sum() == 0
+    some = [0, 200, 511]
+    k64, v64 = unpack(k[:, some], kind), unpack(v[:, some], kind)
+    for i in sorted({0, m // 2, m - 1}):
+        visible = np.arange(n) <= n - m + i
+        want, tol = attend64(unpack(q[i, some], kind), k64, v64, visible)
+        near(got[i, some], want, tol, attend64(unpack(q[i, some], kind), k64, v64, visible)[0], kind)
