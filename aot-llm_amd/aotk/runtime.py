@@ -273,22 +273,29 @@ LOGITS_RULE_DTYPE = np.dtype([("repetition", "<f4"), ("presence", "<f4"), ("freq
 NO_TOKEN = 0xFFFFFFFF  # the pick of a row whose rules leave no token
 
 
-def _dev(a, dtype):
+def _typed(a, dtype):
     a = np.ascontiguousarray(a)
     if a.dtype != dtype:
         raise TypeError(f"expected {dtype} values, got {a.dtype}")
-    return DeviceBuffer.from_numpy(a)
+    return a
+
+
+def _holds(a, n, what):
+    """The kernels read n values of the array, whatever its size is."""
+    if a.size < n:
+        raise ValueError(what)
 
 
 def attention_sinks(q, k_cache, v_cache, n_head, n_kv_head, head_dim, ctx, layer, pos0, m, window, n_sink, kind=abi.F32):
     """Attention of m rows over a sliding window and the first n_sink
     positions (aotk_attention_sinks); bf16 arrays as uint16 bits."""
     t = FLOAT_DTYPES[kind]
-    dq, dk, dv = _dev(q, t), _dev(k_cache, t), _dev(v_cache, t)
+    arrays = [_typed(a, t) for a in (q, k_cache, v_cache)]
     n = m * n_head * head_dim
-    assert n * t.itemsize <= dq.nbytes, "q is smaller than its rows"
-    need = (layer + 1) * ctx * n_kv_head * head_dim * t.itemsize
-    assert need <= dk.nbytes and need <= dv.nbytes, "a cache is smaller than its layers"
+    _holds(arrays[0], n, "q is smaller than its rows")
+    for a in arrays[1:]:
+        _holds(a, (layer + 1) * ctx * n_kv_head * head_dim, "a cache is smaller than its layers")
+    dq, dk, dv = (DeviceBuffer.from_numpy(a) for a in arrays)
     out = DeviceBuffer(n * t.itemsize)
     abi.check(_lib().aotk_attention_sinks(out.ptr, dq.ptr, dk.ptr, dv.ptr, kind, n_head, n_kv_head, head_dim, ctx, layer,
                                           pos0, m, window, n_sink))
@@ -302,13 +309,15 @@ def attention_shared(q, k_prefix, v_prefix, k_tail, v_tail, n_head, n_kv_head, h
     t = FLOAT_DTYPES[kind]
     lens = np.ascontiguousarray(tail_len, np.uint32)
     nr = None if rows is None else np.ascontiguousarray(rows, np.uint32)
-    assert nr is None or nr.size == lens.size, "tail_len and rows differ in length"
+    if nr is not None and nr.size != lens.size:
+        raise ValueError("tail_len and rows differ in length")
     total = lens.size if nr is None else int(nr.sum(dtype=np.uint64))
-    bufs = [_dev(a, t) for a in (q, k_prefix, v_prefix, k_tail, v_tail)]
+    arrays = [_typed(a, t) for a in (q, k_prefix, v_prefix, k_tail, v_tail)]
     n, kv = total * n_head * head_dim, n_kv_head * head_dim
-    assert n * t.itemsize <= bufs[0].nbytes, "q is smaller than its rows"
-    for b, need in zip(bufs[1:], [prefix_ctx] * 2 + [lens.size * tail_ctx] * 2):
-        assert (layer + 1) * need * kv * t.itemsize <= b.nbytes, "a cache is smaller than its layers"
+    _holds(arrays[0], n, "q is smaller than its rows")
+    for a, positions in zip(arrays[1:], [prefix_ctx] * 2 + [lens.size * tail_ctx] * 2):
+        _holds(a, (layer + 1) * positions * kv, "a cache is smaller than its layers")
+    bufs = [DeviceBuffer.from_numpy(a) for a in arrays]
     out = DeviceBuffer(n * t.itemsize)
     abi.check(_lib().aotk_attention_shared(out.ptr, *[b.ptr for b in bufs], kind, n_head, n_kv_head, head_dim, prefix_ctx,
                                            n_prefix, tail_ctx, layer, lens.size, _np_ptr(lens),
@@ -348,14 +357,20 @@ def allowed_mask(tokens, vocab):
     return np.packbits(bits, bitorder="little").view("<u4")
 
 
-def _rules(out_ptr, logits_ptr, kind, rows, vocab, stride, rules, masks, tokens_ptr):
+def _rules_host(rules, masks, rows, vocab):
+    """The host arrays of a call: logits_rules_table's and the masks."""
     table, hist, ids, vals = logits_rules_table(rules)
-    assert len(table) == rows, "one dict of rules per row"
+    if len(table) != rows:
+        raise ValueError(f"one dict of rules per row: {len(table)} for {rows} rows")
     masks = np.zeros((0, (vocab + 31) // 32), np.uint32) if masks is None else np.ascontiguousarray(masks, np.uint32)
-    masks = masks.reshape(-1, (vocab + 31) // 32)
+    return table, hist, ids, vals, masks.reshape(-1, (vocab + 31) // 32)
+
+
+def _rules(out_ptr, logits_ptr, kind, rows, vocab, host, tokens_ptr):
+    table, hist, ids, vals, masks = host
     bufs = [DeviceBuffer.from_numpy(a) if a.size else None for a in (hist, ids, vals, masks)]
     ptr = [b.ptr if b else None for b in bufs]
-    abi.check(_lib().aotk_logits_rules(out_ptr, logits_ptr, kind, rows, vocab, stride, _np_ptr(table), ptr[0], hist.size,
+    abi.check(_lib().aotk_logits_rules(out_ptr, logits_ptr, kind, rows, vocab, vocab, _np_ptr(table), ptr[0], hist.size,
                                        ptr[1], ptr[2], ids.size, ptr[3], len(masks), tokens_ptr))
 
 
@@ -364,11 +379,12 @@ def logits_rules(logits, rules, masks=None, kind=abi.F32):
     [rows][vocab], `rules` one dict per row (logits_rules_table), `masks`
     rows of 32-token words (allowed_mask)."""
     t = FLOAT_DTYPES[kind]
-    logits = np.ascontiguousarray(logits)
+    logits = _typed(logits, t)
     rows, vocab = logits.shape
-    dx = _dev(logits, t)
+    host = _rules_host(rules, masks, rows, vocab)
+    dx = DeviceBuffer.from_numpy(logits)
     out, tok = DeviceBuffer(dx.nbytes), DeviceBuffer(4 * rows)
-    _rules(out.ptr, dx.ptr, kind, rows, vocab, vocab, rules, masks, tok.ptr)
+    _rules(out.ptr, dx.ptr, kind, rows, vocab, host, tok.ptr)
     return out.to_numpy(t).reshape(rows, vocab), tok.to_numpy(np.uint32)
 
 
@@ -506,9 +522,10 @@ class State:
         `mask` one row of allowed tokens (allowed_mask). Returns the greedy
         pick, NO_TOKEN where no token is left."""
         p = abi.check_ptr(_lib().aotk_logits_dev(self.h))
-        tok = DeviceBuffer(4)
         rule = dict(rule, mask=rule.get("mask", -1 if mask is None else 0))
-        _rules(p, p, abi.F32, 1, self.vocab, self.vocab, [rule], mask, tok.ptr)
+        host = _rules_host([rule], mask, 1, self.vocab)
+        tok = DeviceBuffer(4)
+        _rules(p, p, abi.F32, 1, self.vocab, host, tok.ptr)
         return int(tok.to_numpy(np.uint32)[0])
 
     def sample(self, sampler, recent=()):

@@ -139,3 +139,37 @@ def test_the_wrappers_refuse_short_arrays_and_other_types():
     z = np.zeros((1, 4, 1, 64), np.float32)
     with pytest.raises(TypeError, match="float16"):
         runtime.attention_sinks(z[:, 0], z, z, 1, 1, 64, 4, 0, 3, 1, 0, 0, kind=abi.F16)
+
+
+def f32(*shape):
+    return np.zeros(shape, np.float32)
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(q=f32(4, 4, 64)), "q is smaller"), (dict(k=f32(2, 19, 2, 64)), "a cache is smaller"),
+    (dict(v=f32(1, 20, 2, 64)), "a cache is smaller"), (dict(layer=2), "a cache is smaller"), (dict(m=6), "q is smaller"),
+], ids=lambda x: None)
+def test_sinks_of_short_arrays(change, what):
+    a = dict(q=f32(5, 4, 64), k=f32(2, 20, 2, 64), v=f32(2, 20, 2, 64), n_head=4, n_kv_head=2, head_dim=64, ctx=20, layer=1, pos0=10,
+             m=5, window=8, n_sink=2)
+    with pytest.raises(ValueError, match=what):
+        runtime.attention_sinks(*{**a, **change}.values())
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(q=f32(5, 4, 64)), "q is smaller"), (dict(kp=f32(2, 29, 2, 64)), "a cache is smaller"),
+    (dict(vp=f32(1, 30, 2, 64)), "a cache is smaller"), (dict(kt=f32(2, 2, 10, 2, 64)), "a cache is smaller"),
+    (dict(vt=f32(2, 3, 9, 2, 64)), "a cache is smaller"), (dict(layer=2), "a cache is smaller"),
+    (dict(rows=[1, 2, 4]), "q is smaller"), (dict(rows=[3, 3]), "differ in length"), (dict(rows=[1, 2, 3, 0]), "differ in length"),
+], ids=lambda x: None)
+def test_shared_of_short_arrays(change, what):
+    a = dict(q=f32(6, 4, 64), kp=f32(2, 30, 2, 64), vp=f32(2, 30, 2, 64), kt=f32(2, 3, 10, 2, 64), vt=f32(2, 3, 10, 2, 64), n_head=4,
+             n_kv_head=2, head_dim=64, prefix_ctx=30, n_prefix=30, tail_ctx=10, layer=1, tail_len=[5, 10, 3], rows=[1, 2, 3])
+    with pytest.raises(ValueError, match=what):
+        runtime.attention_shared(*{**a, **change}.values())
+
+
+def test_rules_of_fewer_dicts_than_rows():
+    for n in (2, 4):
+        with pytest.raises(ValueError, match="one dict"):
+            runtime.logits_rules(f32(3, 100), [{}] * n)
