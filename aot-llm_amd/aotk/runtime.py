@@ -357,13 +357,26 @@ def allowed_mask(tokens, vocab):
     return np.packbits(bits, bitorder="little").view("<u4")
 
 
+def _mask_words(masks, words):
+    """Masks as rows of `words` 32-bit words (one row may come as a vector)."""
+    if masks is None or np.size(masks) == 0:
+        return np.zeros((0, words), np.uint32)
+    masks = np.atleast_2d(masks)
+    if masks.ndim != 2 or masks.shape[1] != words:
+        raise ValueError(f"masks are rows of {words} words, got {masks.shape}")
+    if masks.dtype == np.int32:
+        masks = np.ascontiguousarray(masks).view(np.uint32)
+    if masks.dtype.kind not in "iu" or masks.dtype.itemsize < 4 or (masks < 0).any() or (masks > 0xFFFFFFFF).any():
+        raise TypeError(f"masks are 32-bit words, got {masks.dtype}")
+    return np.ascontiguousarray(masks, np.uint32)
+
+
 def _rules_host(rules, masks, rows, vocab):
     """The host arrays of a call: logits_rules_table's and the masks."""
     table, hist, ids, vals = logits_rules_table(rules)
     if len(table) != rows:
         raise ValueError(f"one dict of rules per row: {len(table)} for {rows} rows")
-    masks = np.zeros((0, (vocab + 31) // 32), np.uint32) if masks is None else np.ascontiguousarray(masks, np.uint32)
-    return table, hist, ids, vals, masks.reshape(-1, (vocab + 31) // 32)
+    return table, hist, ids, vals, _mask_words(masks, (vocab + 31) // 32)
 
 
 def _rules(out_ptr, logits_ptr, kind, rows, vocab, host, tokens_ptr):

@@ -173,3 +173,22 @@ def test_rules_of_fewer_dicts_than_rows():
     for n in (2, 4):
         with pytest.raises(ValueError, match="one dict"):
             runtime.logits_rules(f32(3, 100), [{}] * n)
+
+
+@pytest.mark.parametrize("masks", [np.ones((1, 64), bool), np.ones((2, 64), np.float32), np.ones((1, 64), np.uint8),
+                                   np.ones((2, 3), np.uint32), np.ones(4, np.uint32), np.ones((1, 2, 2), np.uint32), [[1, -1]]],
+                         ids=lambda m: f"{np.asarray(m).dtype}{np.asarray(m).shape}")
+def test_rules_of_masks_that_are_not_rows_of_words(masks):
+    """64 tokens are two words: a truth value or a byte per token, or the words
+    of another vocabulary, would be read as masks of something else."""
+    with pytest.raises((TypeError, ValueError), match="32-bit words|rows of 2 words"):
+        runtime.logits_rules(f32(2, 64), [{"mask": 0}] * 2, masks)
+
+
+def test_rules_of_masks_as_words():
+    words = np.array([[1, 2], [0xFFFFFFFF, 0]], np.uint32)
+    for masks in (words, words.view(np.int32), words.tolist(), words.astype(np.int64)):
+        assert np.array_equal(runtime._rules_host([{}], masks, 1, 64)[4], words)
+    assert np.array_equal(runtime._rules_host([{}], words[0], 1, 64)[4], words[:1])
+    for none in (None, [], np.zeros((0, 2), np.uint32)):
+        assert runtime._rules_host([{}], none, 1, 64)[4].shape == (0, 2)
