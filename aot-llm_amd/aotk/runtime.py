@@ -535,8 +535,12 @@ class State:
         `mask` one row of allowed tokens (allowed_mask). Returns the greedy
         pick, NO_TOKEN where no token is left."""
         p = abi.check_ptr(_lib().aotk_logits_dev(self.h))
-        rule = dict(rule, mask=rule.get("mask", -1 if mask is None else 0))
-        host = _rules_host([rule], mask, 1, self.vocab)
+        row = -1 if mask is None else 0
+        if rule.get("mask", row) != row:
+            raise ValueError(f"a rule with mask {rule['mask']} beside {'no' if mask is None else 'a'} mask of the state")
+        host = _rules_host([dict(rule, mask=row)], mask, 1, self.vocab)
+        if len(host[4]) != row + 1:
+            raise ValueError("the mask is one row")
         tok = DeviceBuffer(4)
         _rules(p, p, abi.F32, 1, self.vocab, host, tok.ptr)
         return int(tok.to_numpy(np.uint32)[0])

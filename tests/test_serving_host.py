@@ -173,3 +173,28 @@ def test_a_launch_that_fails_is_reported_after_the_others_have_ended(stand_in):
                 assert hip.hh_queued(stream) == 0, (name, i, "launches that nothing has waited for")
             assert call() == 0, (name, lib.aotk_last_error())
     """)
+
+
+def test_a_states_mask_beside_a_rule_that_names_one(stand_in):
+    """apply_rules takes the mask as its argument: a rule of a batch that says
+    otherwise is refused, not followed."""
+    run(stand_in, """
+        spec = aotk.configs.build("tiny-q4km")
+        st = aotk.State(aotk.Model(spec, seed=3), 32, 8)
+        mask = aotk.allowed_mask([3], spec.d["vocab"])
+        for rule, m in (({}, None), ({}, mask), ({"mask": 0}, mask), ({"mask": -1}, None)):
+            st.apply_rules(rule, m)
+        for rule, m in (({"mask": -1}, mask), ({"mask": 0}, None), ({"mask": 2}, mask)):
+            try:
+                st.apply_rules(rule, m)
+            except ValueError as e:
+                assert "mask" in str(e)
+            else:
+                raise AssertionError((rule, m is not None))
+        try:
+            st.apply_rules({}, np.stack([mask, mask]))
+        except ValueError as e:
+            assert "one row" in str(e)
+        else:
+            raise AssertionError("two masks")
+    """)
