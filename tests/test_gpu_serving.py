@@ -825,3 +825,36 @@ def test_large_values_overflow_no_earlier_than_the_formula(aotk, kind, hd, m):
         visible = np.arange(n) <= n - m + i
         want, tol = attend64(unpack(q[i, some], kind), k64, v64, visible)
         near(got[i, some], want, tol, attend64(unpack(q[i, some], kind), k64, v64, visible)[0], kind)
+
+
+# -------------------------------------------------------- the largest counts
+@KINDS
+@pytest.mark.parametrize("nkv", [16384, 1, 128])
+def test_the_most_heads(aotk, kind, nkv):
+    """16384 query heads, each with its own keys or sharing them; a sample."""
+    nh, hd, ctx, m = 16384, 64, 70, 3
+    rng = np.random.default_rng(nkv)
+    q = pack(rng.standard_normal((m, nh, hd), np.float32), kind)
+    k, v = (pack(rng.standard_normal((ctx, nkv, hd), np.float32), kind) for _ in range(2))
+    got = aotk.attention_sinks(q, k, v, nh, nkv, hd, ctx, 0, ctx - m, m, 40, 2, kind).reshape(q.shape)
+    some = [0, 1, 127, 128, 8191, 8192, 16255, 16383]
+    kv = [h * nkv // nh for h in some]
+    k64, v64 = unpack(k[:, kv], kind), unpack(v[:, kv], kind)
+    check_rows(got[:, some], unpack(q[:, some], kind), [(k64, v64, sinks_visible(ctx, ctx - m + i, 40, 2)) for i in range(m)], kind)
+
+
+def test_the_most_sequences(aotk):
+    """65535 sequences behind one prefix, tails of 0 to 2; a sample."""
+    nh, nkv, hd, n = 2, 1, 64, 65535
+    rng = np.random.default_rng(50)
+    tail_len = np.arange(n) % 3
+    q = rng.standard_normal((n, nh, hd), np.float32)
+    kp, vp = rng.standard_normal((2, 1, 37, nkv, hd), np.float32)
+    kt, vt = rng.standard_normal((2, 1, n, 2, nkv, hd), np.float32)
+    got = aotk.attention_shared(q, kp, vp, kt, vt, nh, nkv, hd, 37, 37, 2, 0, tail_len, None, F32).reshape(q.shape)
+    for b in [0, 1, 2, 63, 64, 65, 4095, 32767, 65471, 65472, 65533, 65534]:
+        k, v = (np.concatenate([p[0], t[0, b, :tail_len[b]]]).astype(np.float64) for p, t in ((kp, kt), (vp, vt)))
+        check_rows(got[b:b + 1], q[b:b + 1].astype(np.float64), [(k, v, np.ones(len(k), bool))], F32)
+    # every row, by the sum of its weights: all values equal
+    one = aotk.attention_shared(q, kp, np.ones_like(vp), kt, np.ones_like(vt), nh, nkv, hd, 37, 37, 2, 0, tail_len, None, F32)
+    assert np.abs(one - 1).max() <= 39 * 4 * U
