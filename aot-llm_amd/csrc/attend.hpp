@@ -14,12 +14,16 @@
 // accumulator layout of S^T is, up to the order of the keys, the operand layout
 // of P^T in O^T = V^T P^T. So the weights go from the first product to the
 // second in registers, and only V's operand is read in that order of keys.
-// 16-bit weights go into the second product in the caches' type. Up to 32 rows
-// as two parts, rounded and rest: bound by memory, the product of the rest is free
-// (one row, 32784 bf16 keys: 41.0 and 41.4 us, error 2.5e-3 and 1.6e-3). More rows
-// are bound by the products: there rounded, half a step each against values that
-// are themselves rounded so. The sum takes them rounded too, so that equal values
-// stay what they are (8192 rows: 492 us with the sum before rounding, 490 so).
+// 16-bit weights go into the second product in the caches' type. Up to 32 rows of a
+// sequence (positions x heads of a group; 16 with heads of 256) as two parts, rounded
+// and rest: bound by memory, the product of the rest is free (one row, 32784 bf16 keys: 41.0 and 41.4 us, error 2.5e-3 and 1.6e-3). The
+// prefix's blocks, over the rows of all such sequences, keep both parts too, so
+// that a row is as exact in a large batch as alone (bf16, a call of 64 sequences
+// behind 8192 53.7 us rounded and 54.6 so, error 2.3e-3 and 1.7e-3; where the prefix
+// outweighs the tails, 64 behind 30000: 83 and 95 us). Sequences of more rows are
+// bound by the products: there rounded, half a step each against values that are
+// themselves rounded so. The sum takes them rounded too, so that equal values stay
+// what they are (8192 rows: 492 us with the sum before rounding, 490 so).
 //
 // A block takes one kv head, a tile of rows (all query heads of the group x
 // positions, heads fastest) and a run of key tiles. Where runs are cut or a
@@ -610,7 +614,8 @@ struct WideShape {
     static constexpr size_t lds_bytes() { return 2 * (size_t)NK * (KS + VS) * ESZ + 6 * sizeof(uint32_t); }
 };
 
-template <int KIND, int D, int NW>
+// TWO: 16-bit weights in two parts.
+template <int KIND, int D, int NW, bool TWO>
 __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, uint8_t *lds) {
     typedef WideShape<KIND, D> S;
     typedef typename AttElem<KIND>::elem E;
@@ -663,16 +668,27 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
         }
     };
     // into the buffer; values past the tile's end become 0, and in a tile
-    // that rows see differently those not finite do, their keys noted
+    // that rows see differently, or whose weights have two parts, those not
+    // finite do, their keys noted
     auto put = [&](const AttTile<E> &x, int buf, int slot) {
+        bool apart = x.ragged;
+        if constexpr (TWO) {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 top = {0, 0};
+#pragma unroll
+            for (int e = 0; e < NCH; e++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, sv[e][c] & 0x7FFF7FFFu));
+            apart |= __any(!AttElem<KIND>::finite(top[0]) || !AttElem<KIND>::finite(top[1]));
+        }
 #pragma unroll
         for (int e = 0; e < NCH; e++) {
             const int row = srow + e * RSTEP;
-            if (x.n < NK || x.ragged) {
+            if (x.n < NK || apart) {
                 u32x4 &y = sv[e];
                 bool bad = false;
                 if ((uint32_t)row >= x.n) y = u32x4{0, 0, 0, 0};
-                else if (x.ragged)
+                else if (apart)
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         if constexpr (F32) {
@@ -744,7 +760,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
         // waves a SIMD take turns by themselves.)
         constexpr int P = NK / 32, KG = S::QR / 4;
         f32x16 sc[P];
-        uint32_t p16[P * 8];  // 16 bits: the weights, two a word, in sc's order
+        uint32_t p16[P * 8], p16_rest[P * 8];  // 16 bits: the weights, two a word, in sc's order
         u32x4 kf[2][4], vf[2][VG];
         const E *const krow = lk + (buf * NK + n) * S::KS + (F32 ? 4 * h : 8 * h);
         auto read_k = [&](int kb, int gi) {
@@ -805,7 +821,12 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                     part[i % 4] += x + y;
                 } else {
                     p16[i] = AttElem<KIND>::pair(x, y);
-                    part[i % 4] = AttElem<KIND>::add_pair(p16[i], part[i % 4]);
+                    if constexpr (TWO) {
+                        p16_rest[i] = AttElem<KIND>::pair(x - AttElem<KIND>::first(p16[i]), y - AttElem<KIND>::second(p16[i]));
+                        part[i % 4] += x + y;
+                    } else {
+                        part[i % 4] = AttElem<KIND>::add_pair(p16[i], part[i % 4]);
+                    }
                 }
             }
             sum += (part[0] + part[1]) + (part[2] + part[3]);
@@ -819,6 +840,11 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
                 const u32x4 p = {p16[vi * 4], p16[vi * 4 + 1], p16[vi * 4 + 2], p16[vi * 4 + 3]};
 #pragma unroll
                 for (int c = 0; c < S::NA; c++) acc[c] = AttElem<KIND>::mma32(vf[vi & 1][c], p, acc[c]);
+                if constexpr (TWO) {
+                    const u32x4 r = {p16_rest[vi * 4], p16_rest[vi * 4 + 1], p16_rest[vi * 4 + 2], p16_rest[vi * 4 + 3]};
+#pragma unroll
+                    for (int c = 0; c < S::NA; c++) acc[c] = AttElem<KIND>::mma32(vf[vi & 1][c], r, acc[c]);
+                }
             }
         };
         read_k(0, 0);
@@ -835,7 +861,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
             if (vi + 1 < VN) read_v(buf, vi + 1, vf[(vi + 1) & 1]);
             values(vi);
         }
-        if (x.ragged) {
+        if (x.ragged || TWO) {
             for (int half = 0; half < NK / 32; half++) {
                 uint32_t bad = __builtin_amdgcn_readfirstlane(l_bad[slot][half]);
                 const AttSees sees(w, x, rel);
@@ -846,7 +872,7 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
 #pragma unroll
                     for (int i = 0; i < P * 16; i++) {
                         float y;
-                        if constexpr (F32) y = sc[0][i];
+                        if constexpr (F32 || TWO) y = sc[i / 16][i % 16];
                         else y = i % 2 ? AttElem<KIND>::second(p16[i / 2]) : AttElem<KIND>::first(p16[i / 2]);
                         pv = i == (c / 32) * 16 + c % 32 / 8 * 4 + c % 4 ? y : pv;
                     }
@@ -910,10 +936,10 @@ __device__ __forceinline__ void attend_wide(const AttendLaunch &a, bool prefix, 
 // for the matrix cores, the tails' few rows for memory, and neither alone fills
 // the chip. P and O: 16-row tiles of attend_narrow (1, 2) or 32-row waves of
 // attend_wide (3: two waves, 4: four).
-template <int KIND, int D, int SHAPE, int NW>
+template <int KIND, int D, int SHAPE, int NW, bool TWO>
 __device__ __forceinline__ void attend_shape(const AttendLaunch &a, bool prefix, uint8_t *lds) {
     if constexpr (SHAPE <= 2) attend_narrow<KIND, D, NW, SHAPE>(a, prefix, lds);
-    else attend_wide<KIND, D, NW>(a, prefix, lds);
+    else attend_wide<KIND, D, NW, TWO>(a, prefix, lds);
 }
 
 constexpr int att_waves(int p) { return p == 3 ? 2 : 4; }
@@ -929,10 +955,10 @@ __global__ __launch_bounds__(64 * att_waves(P), D == 256 || P == 3 ? 1 : 2) void
     extern __shared__ __align__(16) uint8_t lds[];
     const bool prefix = blockIdx.x < a.prefix_blocks;
     if constexpr (P == O) {
-        attend_shape<KIND, D, P, att_waves(P)>(a, prefix, lds);
+        attend_shape<KIND, D, P, att_waves(P), false>(a, prefix, lds);
     } else {
-        if (prefix) attend_shape<KIND, D, P, att_waves(P)>(a, true, lds);
-        else attend_shape<KIND, D, O, att_waves(P)>(a, false, lds);
+        if (prefix) attend_shape<KIND, D, P, att_waves(P), KIND != AOTK_F32>(a, true, lds);
+        else attend_shape<KIND, D, O, att_waves(P), false>(a, false, lds);
     }
 }
 
@@ -1027,6 +1053,9 @@ static void att_launch_d(int p, int o, const AttendLaunch &a, uint32_t blocks, h
         if constexpr (D < 256) return att_start<KIND, D, 2, 2>(a, blocks, s);
         break;
     case 3 * 8 + 1: return att_start<KIND, D, 3, 1>(a, blocks, s);
+    case 3 * 8 + 2:
+        if constexpr (KIND != AOTK_F32 && D < 256) return att_start<KIND, D, 3, 2>(a, blocks, s);
+        break;
     case 3 * 8 + 3: return att_start<KIND, D, 3, 3>(a, blocks, s);
     case 4 * 8 + 1: return att_start<KIND, D, 4, 1>(a, blocks, s);
     case 4 * 8 + 2:

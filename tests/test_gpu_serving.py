@@ -858,3 +858,58 @@ def test_the_most_sequences(aotk):
     # every row, by the sum of its weights: all values equal
     one = aotk.attention_shared(q, kp, np.ones_like(vp), kt, np.ones_like(vt), nh, nkv, hd, 37, 37, 2, 0, tail_len, None, F32)
     assert np.abs(one - 1).max() <= 39 * 4 * U
+
+
+# ------------------------------------------- decode rows in batches of any size
+def near_equal_weights(kind, n, hd):
+    """Two sets of keys, values 1 and -1, whose weights differ by less than half
+    a step of the type: q [hd], k and v [n, 1, hd]."""
+    q, k, v = np.zeros(hd), np.zeros((n, 1, hd)), np.ones((n, 1, hd))
+    q[0] = 1
+    k[::2, 0, 0] = {BF16: 0.0015, F16: 2e-4}[kind] * np.sqrt(hd)
+    v[1::2] = -1
+    return pack(q, kind), pack(k, kind), pack(v, kind)
+
+
+@pytest.mark.parametrize("kind", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("nh,hd,batch", [(4, 64, 9), (8, 128, 5), (16, 128, 3), (8, 128, 40), (32, 64, 8), (20, 128, 70), (8, 256, 5),
+                                         (16, 256, 40), (20, 128, 3), (24, 64, 2), (32, 128, 2), (16, 128, 1), (8, 64, 4)], ids=str)
+def test_weights_of_decode_rows_keep_both_parts_in_any_batch(aotk, kind, nh, hd, batch):
+    """A sequence's row is as exact in a large batch as alone: also the prefix's
+    blocks, over all sequences' rows, take 16-bit weights in two parts."""
+    e, n_prefix, n_tail = HALF_STEP[kind], 150, 10
+    q, k, v = near_equal_weights(kind, n_prefix + n_tail, hd)
+    q = np.broadcast_to(q, (batch, nh, hd))
+    tails = [np.broadcast_to(x[n_prefix:], (batch, n_tail, 1, hd)) for x in (k, v)]
+    got = aotk.attention_shared(q, k[:n_prefix], v[:n_prefix], *tails, nh, 1, hd, n_prefix, n_prefix, n_tail, 0, [n_tail] * batch, None,
+                                kind)
+    got = unpack(got, kind).reshape(batch, nh, hd)
+    q64, k64, v64 = (unpack(x, kind) for x in (q, k, v))
+    want, tol = attend64(q64[0], k64, v64, np.ones(n_prefix + n_tail, bool))
+    s = k64[:, 0, 0] / np.sqrt(hd)
+    w = np.exp(s - s.max())
+    rounded = np.abs((unpack(pack(w, kind), kind) @ v64[:, 0, 0]) / w.sum() - want)
+    tol = tol + 1.01 * e * e + (len(s) * 2.0 ** -31 if kind == F16 else 0)
+    assert (rounded > 2 * (tol + np.abs(want) * e)).all()
+    for b in range(batch):
+        near(got[b], want, tol, 0.0, kind)
+
+
+@KINDS
+@pytest.mark.parametrize("nh,hd,batch", [(4, 64, 9), (8, 128, 5), (16, 128, 40), (8, 256, 5), (16, 256, 40), (20, 128, 3), (32, 64, 2),
+                                         (24, 128, 9)], ids=str)
+def test_infinite_values_of_the_prefix_in_decode_batches(aotk, kind, nh, hd, batch):
+    """Infinities stay infinities, two of both signs and a NaN become NaN, in
+    their dimensions alone; also in the prefix's last, short tile."""
+    rng = np.random.default_rng(60)
+    n_prefix, n_tail = 330, 3
+    q = pack(rng.standard_normal((batch, nh, hd)), kind)
+    k, v = rng.standard_normal((2, 1, n_prefix, 1, hd))
+    for j, d, x in [(10, 5, np.inf), (99, 6, -np.inf), (20, 7, np.inf), (170, 7, -np.inf), (140, 9, np.nan), (329, 12, np.inf),
+                    (200, 63, -np.inf), (64, 0, np.inf), (65, 0, np.inf)]:
+        v[0, j, 0, d] = x
+    kp, vp = pack(k, kind), pack(v, kind)
+    kt, vt = (pack(rng.standard_normal((1, batch, n_tail, 1, hd)), kind) for _ in range(2))
+    got = aotk.attention_shared(q, kp, vp, kt, vt, nh, 1, hd, n_prefix, n_prefix, n_tail, 0, [n_tail] * batch, None, kind)
+    with np.errstate(invalid="ignore"):
+        check_rows(got, unpack(q, kind), shared_rows(kp, vp, kt, vt, n_prefix, [n_tail] * batch, [1] * batch, kind, 0), kind)
