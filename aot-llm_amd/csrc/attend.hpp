@@ -299,7 +299,7 @@ template <int KIND, int D>
 struct NarrowShape {
     static constexpr bool F32 = KIND == AOTK_F32;
     static constexpr int NK = F32 ? 16 : 32;          // keys of a tile
-    static constexpr int KR = F32 ? D / 16 : D / 16;  // 16-byte loads of K per lane
+    static constexpr int KR = D / 16;                 // 16-byte loads of K per lane
     static constexpr int VL = F32 ? D / 64 : (D == 256 ? 2 : 1);  // loads per key of V
     static constexpr int VK = F32 ? 4 : 8;            // keys of V per lane
     static constexpr int CW = F32 ? 4 : (D == 64 ? 4 : 8);  // dimensions per load of V

@@ -249,6 +249,8 @@ int aotk_attention(float *out_dev, const float *q_dev, const float *k_cache_dev,
  * counterpart in the reference. Their element kind is AOTK_F32, AOTK_F16 or
  * AOTK_BF16, the same for all tensors of a call; scores, softmax statistics
  * and sums are f32, and results are rounded once to the kind, to nearest.
+ * (Softmax weights are rounded to an f16 or bf16 kind too where a sequence has
+ * more than 32 rows x heads per kv head, 16 for head_dim 256.)
  * Pointers need the alignment of one element. Outputs must not overlap inputs
  * (aotk_logits_rules may write its logits in place). Like every call here they
  * run on the library's stream and return when the result is there: what other
@@ -272,8 +274,9 @@ int aotk_attention_sinks(void *out_dev, const void *q_dev, const void *k_cache_d
 /* Attention of a batch of sequences that share a prefix, whose keys and
  * values are read once for all of them.
  *   k_prefix_dev, v_prefix_dev: [n_layer][prefix_ctx][kv_dim], the first
- *     n_prefix positions hold the prefix (e.g. a state's cache after
- *     aotk_prefix_load);
+ *     n_prefix positions hold the prefix (e.g. what aotk_kv_download reads
+ *     from a state after aotk_prefix_load, copied to the device: prefix_ctx is
+ *     its n_pos);
  *   k_tail_dev, v_tail_dev: [n_layer][batch][tail_ctx][kv_dim], sequence b
  *     holds tail_len_host[b] <= tail_ctx positions of its own;
  *   rows_host[b] rows of sequence b (null: one each, the decode step), packed

@@ -913,3 +913,18 @@ def test_infinite_values_of_the_prefix_in_decode_batches(aotk, kind, nh, hd, bat
     got = aotk.attention_shared(q, kp, vp, kt, vt, nh, 1, hd, n_prefix, n_prefix, n_tail, 0, [n_tail] * batch, None, kind)
     with np.errstate(invalid="ignore"):
         check_rows(got, unpack(q, kind), shared_rows(kp, vp, kt, vt, n_prefix, [n_tail] * batch, [1] * batch, kind, 0), kind)
+
+
+def test_a_states_cache_as_the_prefix(aotk):
+    """What kv_download reads is the prefix of continuations, layer by layer."""
+    d = aotk.configs.build("tiny-q4km").d
+    nh, nkv, hd, n, n_pos = d["n_head"], d["n_kv_head"], d["head_dim"], 12, 15
+    st = aotk.State(aotk.Model(aotk.configs.build("tiny-q4km"), seed=3), 32, 8)
+    st.prompt(aotk.configs.prompt_tokens(1, n, d["vocab"]), batch=8)
+    kp, vp = (x.reshape(d["n_layer"], n_pos, nkv, hd) for x in st.kv_download(n_pos))
+    rng = np.random.default_rng(70)
+    q = rng.standard_normal((3, nh, hd)).astype(np.float32)
+    kt, vt = rng.standard_normal((2, d["n_layer"], 3, 4, nkv, hd)).astype(np.float32)
+    for layer in range(d["n_layer"]):
+        got = aotk.attention_shared(q, kp, vp, kt, vt, nh, nkv, hd, n_pos, n, 4, layer, [4, 0, 2])
+        check_rows(got, q.astype(np.float64), shared_rows(kp, vp, kt, vt, n, [4, 0, 2], [1] * 3, F32, layer), F32)
