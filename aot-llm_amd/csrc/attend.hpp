@@ -292,8 +292,8 @@ __device__ __forceinline__ float att_shift(float from, float to) { return from =
 // requested as soon as the scores are formed, its V after the second product.
 // V arrives as a lane's 8 keys x 8 dimensions and is transposed there by byte
 // permutes. The waves' results meet in LDS at the end.
-// One bf16 row, 32 heads over 8 of 128, 32784 keys: 134 MB in 24 us, 5.6 TB/s (a
-// large copy reaches 5.1). One f32 row of 1028 keys: 9.4 us, the latency of one
+// One bf16 row, 32 heads over 8 of 128, 32784 keys: 134 MB in 24.6 us, 5.5 TB/s (a
+// large copy reaches 6.2). One f32 row of 1028 keys: 9.4 us, the latency of one
 // tile from the arguments to the result, of which the memory takes 2.
 template <int KIND, int D>
 struct NarrowShape {

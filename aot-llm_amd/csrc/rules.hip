@@ -12,7 +12,7 @@
 // rules travel in the launch's arguments.
 //
 // One read and one write of the logits bound it: 256 x 262144 bf16, 268 MB, 67 us
-// (4.0 TB/s; a large copy reaches 5.1), 64 x 128256 f32 18 us, 1 x 32000 5.7 us.
+// (4.1 TB/s; a large copy reaches 6.2), 64 x 128256 f32 18 us, 1 x 32000 6.0 us.
 //
 // A block takes slices of RULE_SLICE tokens of one row. What names tokens
 // in list order (history, biases) is turned into per-token tables in LDS:
