@@ -59,8 +59,8 @@ static void att_cut(int kind, int head_dim, const AttendArgs &a, uint64_t na, bo
     // writing and joining their results (f32, for every row) would cost more than
     // the tiles of a run: c runs of T tiles take T / c tile times and c times the
     // traffic of one result. Measured around that optimum (times 0.7 / 1 / 1.5 of
-    // its c): 64 sequences behind 8192 bf16, weights rounded, 56 / 52 / 57 us, 64 f32 rows in a 1024
-    // window 53 / 47 / 54 us. Few rows: runs of one tile a wave at least (of two: 27
+    // its c): 64 sequences behind 8192 bf16, weights rounded, 56 / 52 / 57 us, 64 f32
+    // rows in a 1024 window 53 / 47 / 54 us. Few rows: runs of one tile a wave at least (of two: 27
     // -> 30 us for a 1024 window, one f32 row).
     const bool narrow = p.shape <= 2;
     const double want = 512, least = narrow ? 4 : 1;

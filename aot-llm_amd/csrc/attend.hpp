@@ -15,15 +15,16 @@
 // of P^T in O^T = V^T P^T. So the weights go from the first product to the
 // second in registers, and only V's operand is read in that order of keys.
 // 16-bit weights go into the second product in the caches' type. Up to 32 rows of a
-// sequence (positions x heads of a group; 16 with heads of 256) as two parts, rounded
-// and rest: bound by memory, the product of the rest is free (one row, 32784 bf16 keys: 41.0 and 41.4 us, error 2.5e-3 and 1.6e-3). The
-// prefix's blocks, over the rows of all such sequences, keep both parts too, so
-// that a row is as exact in a large batch as alone (bf16, a call of 64 sequences
-// behind 8192 53.7 us rounded and 54.6 so, error 2.3e-3 and 1.7e-3; where the prefix
-// outweighs the tails, 64 behind 30000: 83 and 95 us). Sequences of more rows are
-// bound by the products: there rounded, half a step each against values that are
-// themselves rounded so. The sum takes them rounded too, so that equal values stay
-// what they are (8192 rows: 492 us with the sum before rounding, 490 so).
+// sequence (positions x heads of a group; 16 with heads of 256) as two parts,
+// rounded and rest: bound by memory, the product of the rest is free (one row,
+// 32784 bf16 keys: 41.0 and 41.4 us, error 2.5e-3 and 1.6e-3). The prefix's blocks,
+// over the rows of all such sequences, keep both parts too, so that a row is as
+// exact in a large batch as alone (bf16, a call of 64 sequences behind 8192 53.7 us
+// rounded and 54.6 so, error 2.3e-3 and 1.7e-3; where the prefix outweighs the tails,
+// 64 behind 30000: 83 and 95 us). Sequences of more rows are bound by the products:
+// there rounded, half a step each against values that are themselves rounded so.
+// The sum takes them rounded too, so that equal values stay what they are (8192
+// rows: 492 us with the sum before rounding, 490 so).
 //
 // A block takes one kv head, a tile of rows (all query heads of the group x
 // positions, heads fastest) and a run of key tiles. Where runs are cut or a
@@ -58,7 +59,7 @@ constexpr float RESCALE = 8.0f;
 // 2^-14 an f16 loses bits, and a long row may have many weights that small beside
 // one large; its values are too small to overflow. The other types hold values as
 // large as f32 itself: at 2^-8 their weights are at most 1, and the sums overflow
-// where those of the formula do. bf16 takes the 2^-8 in the exponent; there it
+// where those of the formula do (values below 2^-118 may lose bits). bf16 takes the 2^-8 in the exponent; there it
 // would cost f32 weights two bits, which are multiplied by it instead.
 template <int KIND>
 constexpr float LIFT = KIND == AOTK_F16 ? 6.0f : (KIND == AOTK_BF16 ? -RESCALE : 0.0f);
